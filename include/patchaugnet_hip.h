@@ -506,6 +506,54 @@ int pa_patch_pairs_fill(int nrec, const int *idx1, const int *near_off, const in
 int pa_knn_mfma_select(const float *a, long lda, int nq_blk, int nr, int dim, int k, const float *ref_rows, const float *query_rows,
                        const float *qnorm, const float *rnorm_max, int q0, int nq_total, float *dist, int64_t *ind, int *flags, pa_stream_t stream);
 
+/* ---- attention with a sliding window over ordered tokens, its norm and rotation, its paged form for one new token --------------
+ * dtype: 0 float32, 1 float16, 2 bfloat16.  Strided tensors are given with the strides (in elements) of their dimensions but the
+ * last, which is contiguous; addresses and strides of the attention entries are multiples of 16 bytes (pa_qk_norm_rotary takes any).
+ * h query heads share hk key heads (h % hk == 0, query head i reads key head i / (h / hk)).  Not in the reference.
+ *
+ * Query i of sequence b stands at position p = start[b] + i (start NULL: 0); key j is in view if j < length[b] (NULL: m), j <= p + right,
+ * and j >= p - left or j < sinks.  left / right -1: no limit.  Queries at p >= length[b] are padding: their output and gradients are 0.
+ * start and length are device arrays, values outside 0..m are clamped. */
+
+/* Norm of every head of q (b,n,h,d) and k (b,n,hk,d) over d, weights qw / kw (d; NULL: 1; w_f32: float32, else of dtype), then the first
+ * 2 axes per elements rotated by pos[b][n][a] freq[a][f]: pairs (i, i + axes per), interleaved: (2 i, 2 i + 1).  pos: ptype 0 int32,
+ * 1 int64, 2 float32, (n, axes) per sequence, pb elements apart (0: shared).  d <= 512.  Outputs contiguous. */
+int pa_qk_norm_rotary(int dtype, int b, int n, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn, long kh,
+                      const void *qw, const void *kw, int w_f32, const void *pos, int ptype, long pb, const float *freq, int axes, int per, float eps,
+                      int interleaved, void *q_out, void *k_out, pa_stream_t stream);
+/* Gradients: gq, gk of the outputs -> dq, dk (contiguous), dqw, dkw (d float32; NULL: not wanted; either wanted: scratch). */
+long pa_qk_norm_rotary_backward_scratch_floats(int b, int n, int d);
+int pa_qk_norm_rotary_backward(int dtype, int b, int n, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn, long kh,
+                               const void *qw, const void *kw, int w_f32, const void *pos, int ptype, long pb, const float *freq, int axes, int per, float eps,
+                               int interleaved, const void *gq, long gqb, long gqn, long gqh, const void *gk, long gkb, long gkn, long gkh, void *dq, void *dk,
+                               float *dqw, float *dkw, float *scratch, pa_stream_t stream);
+
+/* out (b,n,h,d, contiguous) = softmax(scale q k^T over the keys in view) v; q (b,n,h,d), k and v (b,m,hk,d), d a multiple of 8 up to 128.
+ * lse (b,h,n; NULL: not wanted): log2 of the sum of exponentials, for the backward pass.  scratch: as many floats as the function says (0: NULL). */
+long pa_window_attention_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks);
+int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn, long kh,
+                        const void *v, long vb, long vn, long vh, int left, int right, int sinks, float scale, const int *start, const int *length, void *out,
+                        float *lse, float *scratch, pa_stream_t stream);
+/* dq, dk, dv (contiguous) from dout (b,n,h,d) and the forward's out and lse.  Sums in a fixed order: the same bits every time. */
+long pa_window_attention_backward_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks);
+int pa_window_attention_backward(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn,
+                                 long kh, const void *v, long vb, long vn, long vh, const void *out, const float *lse, const void *dout, long gb, long gn, long gh,
+                                 int left, int right, int sinks, float scale, const int *start, const int *length, void *dq, void *dk, void *dv, float *scratch,
+                                 pa_stream_t stream);
+
+/* One new token per sequence: out (b,h,d) for q (b,h,d) at position length[b] - 1 over the cache, whose key j lies in page
+ * table[b][j / page], row j % page, of k_pages / v_pages (pages, page, hk, d).  Keys in view: j >= length - 1 - left or j < sinks.  A table entry
+ * outside 0..pages-1 holds no keys.  length is clamped to 0..width page; an empty sequence gives zeros. */
+long pa_paged_attention_scratch_floats(int b, int h, int hk, int d, int page, int width, int left, int sinks);
+int pa_paged_attention(int dtype, int b, int h, int hk, int d, const void *q, long qb, long qh, const void *k_pages, long kp, long kt, long kh,
+                       const void *v_pages, long vp, long vt, long vh, int pages, int page, const int *table, int width, const int *length, int left, int sinks,
+                       float scale, void *out, float *scratch, pa_stream_t stream);
+/* k, v (b,tokens,hk,d) into the cache: token t < counts[b] (NULL: all) at position starts[b] + t; positions outside the table and pages outside
+ * the pool are skipped. */
+int pa_paged_append(int dtype, int b, int tokens, int hk, int d, const void *k, long kb, long kn, long kh, const void *v, long vb, long vn, long vh, void *k_pages,
+                    long kp, long kt, long kph, void *v_pages, long vp, long vt, long vph, int pages, int page, const int *table, int width, const int *starts,
+                    const int *counts, pa_stream_t stream);
+
 /* ---- the reference's launcher names (group 2) -------------------------------------------------*/
 void furthestsampling_cuda_launcher(int b, int n, int m, const float *dataset, float *temp, int *idxs);
 void gathering_forward_cuda_launcher(int b, int c, int n, int m, const float *points, const int *idx, float *out);

@@ -116,6 +116,12 @@ _SIGS = {
     "pa_linear_x3": "lpipfpi",
     "pa_fp_chain_premul_g16": "ipppplppppiiiipppi",
     "pa_fp_chain_premul_g16h": "ipppplppppiiiippp",
+    "pa_qk_norm_rotary": "iiiiii" + "plll" * 2 + "ppipilpiifipp",
+    "pa_qk_norm_rotary_backward": "iiiiii" + "plll" * 2 + "ppipilpiifi" + "plll" * 2 + "ppppp",
+    "pa_window_attention": "iiiiiii" + "plll" * 3 + "iiifppppp",
+    "pa_window_attention_backward": "iiiiiii" + "plll" * 3 + "pp" + "plll" + "iiifpppppp",
+    "pa_paged_attention": "iiiii" + "pll" + "plll" * 2 + "iipipiifpp",
+    "pa_paged_append": "iiiii" + "plll" * 4 + "iipipp",
 }
 _T = {"i": _I, "f": _F, "p": _P, "l": ctypes.c_long, "d": ctypes.c_double, "q": ctypes.c_ulonglong}
 
@@ -154,7 +160,9 @@ def _load(path):
     l.pa_last_error.restype = ctypes.c_char_p
     l.pa_abi_version.restype = _I
     for name, nargs in (("pa_interpolation_backward_scratch_ints", 3), ("pa_netvlad_scratch_floats", 3), ("pa_afa_scratch_floats", 4), ("pa_fc_scratch_floats", 3), ("pa_afa_rows_scratch_floats", 4), ("pa_pack_weights_f16_halfs", 2),
-                        ("pa_afa_fused_scratch_floats", 3), ("pa_attn_train_scratch_floats", 2), ("pa_sa_attention_f16_scratch_halfs", 4), ("pa_cloud_cellsort_floats", 2)):
+                        ("pa_afa_fused_scratch_floats", 3), ("pa_attn_train_scratch_floats", 2), ("pa_sa_attention_f16_scratch_halfs", 4), ("pa_cloud_cellsort_floats", 2),
+                        ("pa_qk_norm_rotary_backward_scratch_floats", 3), ("pa_window_attention_scratch_floats", 9), ("pa_window_attention_backward_scratch_floats", 9),
+                        ("pa_paged_attention_scratch_floats", 8)):
         getattr(l, name).argtypes = [_I] * nargs
         getattr(l, name).restype = ctypes.c_long
     l.pa_sa_group_window.argtypes, l.pa_sa_group_window.restype = [_I, _I], _I      # thread-local state setter: no stream argument

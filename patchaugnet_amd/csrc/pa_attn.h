@@ -1,0 +1,239 @@
+// Shared device code of the windowed / paged attention kernels (window_attention.hip, window_attention_bwd.hip, paged_attention.hip).
+//
+// All of them multiply with 32 x 32 MFMA tiles and keep the same register layouts:
+//   operand fragment  lane l holds row l % 32, contraction slots 8 (l / 32) + e, e = 0..7 of 16
+//   accumulator       lane l holds column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4, r = 0..15
+// 16-bit types contract 16 slots with one v_mfma_f32_32x32x16; float32 contracts them with eight v_mfma_f32_32x32x2, MFMA e taking slots e and 8 + e.
+//
+// Eight accumulator registers of a lane (r = 8 u .. 8 u + 7) ARE an operand fragment whose slot 8 h + e stands for row 16 u + 4 h + e (e < 4) or
+// 16 u + 8 + 4 h + e - 4: a product computed into registers feeds the next one without leaving them, if the other operand lists its contraction
+// index in the same order (ldt below).
+#pragma once
+#include "pa_common.h"
+
+typedef float pa_f16v __attribute__((ext_vector_type(16)));
+typedef float pa_f8 __attribute__((ext_vector_type(8)));
+typedef float pa_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 pa_bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pa_bf4 __attribute__((ext_vector_type(4)));
+typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pa_h4 __attribute__((ext_vector_type(4)));
+typedef short pa_s4 __attribute__((ext_vector_type(4)));
+typedef u32 pa_u4 __attribute__((ext_vector_type(4), may_alias));
+
+enum { PA_DT_F32 = 0, PA_DT_F16 = 1, PA_DT_BF16 = 2 };
+
+namespace pa_attn {
+
+constexpr int MAXLEN = 1 << 28;          // tokens of a sequence, rows of a key head: their sums and those with a window side stay inside 32 bits
+constexpr int UNBOUNDED = 1 << 29;       // window side without a limit
+constexpr int NOWHERE = 0x7fffffff;      // a position that no key reaches
+
+template <typename T> struct Frag;
+template <> struct Frag<float> { typedef pa_f8 type; };
+template <> struct Frag<_Float16> { typedef pa_h8 type; };
+template <> struct Frag<__bf16> { typedef pa_bf8 type; };
+
+__device__ __forceinline__ void mma(pa_f16v &c, const pa_bf8 &a, const pa_bf8 &b) { c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ void mma(pa_f16v &c, const pa_h8 &a, const pa_h8 &b) { c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ void mma(pa_f16v &c, const pa_f8 &a, const pa_f8 &b)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// value of the lane with the other l / 32
+__device__ __forceinline__ float other_half(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// A tile of rows in LDS: 16-byte chunks, chunk c of row r at place c ^ swz(r).  The swizzle makes both kinds of reads free of bank conflicts for
+// every row width (multiples of 64 bytes): 16 rows at one chunk (operand fragments) and 4 rows at 4 neighbouring chunks (transposed fragments).
+template <typename T, int DT> struct Tile {
+    static constexpr int RB = DT * (int)sizeof(T);           // bytes of a row
+    static constexpr int CH = RB / 16;                       // chunks of a row
+    static constexpr int EC = 16 / (int)sizeof(T);           // elements of a chunk
+
+    __device__ static __forceinline__ int swz(int r)
+    {
+        const int low = (r >> 2) & 3;
+        if (RB % 256 == 0) return ((r & 3) << 2) | low;
+        if (RB % 128 == 0) return ((r & 2) << 1) | low;
+        return low;
+    }
+    __device__ static __forceinline__ int at(int r, int c) { return r * RB + ((c ^ swz(r)) << 4); }
+
+    // operand fragment: row r0 + l % 32, elements 16 kk + 8 (l / 32) ..
+    __device__ static __forceinline__ typename Frag<T>::type ld(const char *s, int r0, int kk)
+    {
+        const int l = threadIdx.x & 63, r = r0 + (l & 31), h = l >> 5;
+        typename Frag<T>::type f;
+        if constexpr (sizeof(T) == 2) {
+            f = *reinterpret_cast<const typename Frag<T>::type *>(s + at(r, 2 * kk + h));
+        } else {
+            const pa_f4 a = *reinterpret_cast<const pa_f4 *>(s + at(r, 4 * kk + 2 * h)), b = *reinterpret_cast<const pa_f4 *>(s + at(r, 4 * kk + 2 * h + 1));
+            f = (pa_f8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        }
+        return f;
+    }
+
+    // transposed fragment: "row" = element c0 + l % 32, contraction slots over the rows r0 .. r0 + 15 in the accumulators' order
+    // (slot 8 h + e: row r0 + 4 h + e, e < 4, or r0 + 8 + 4 h + e - 4).  16-bit: ds_read_b64_tr_b16, where lane s of 16 passes the address of four
+    // elements of row s / 4 and receives one element of each of the four rows.
+    __device__ static __forceinline__ typename Frag<T>::type ldt(const char *s, int r0, int c0)
+    {
+        const int l = threadIdx.x & 63, h = l >> 5;
+        if constexpr (sizeof(T) == 2) {
+            const int q = l & 15, c = c0 + (l & 16) + 4 * (q & 3);
+            const int ra = r0 + 4 * h + (q >> 2), rb = ra + 8;
+            typedef __attribute__((address_space(3))) pa_s4 *lp;
+            const pa_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(s + at(ra, c >> 3) + (c & 4) * 2));
+            const pa_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(s + at(rb, c >> 3) + (c & 4) * 2));
+            typedef short s8 __attribute__((ext_vector_type(8)));
+            const s8 z = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(typename Frag<T>::type, z);
+        } else {
+            pa_f8 f;
+            const int c = c0 + (l & 31);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int r = r0 + 4 * h + (e & 3) + 8 * (e >> 2);
+                f[e] = *reinterpret_cast<const float *>(s + at(r, c >> 2) + (c & 3) * 4);
+            }
+            return f;
+        }
+    }
+};
+
+// eight accumulator registers as an operand fragment (one rounding to the operand type)
+template <typename T> __device__ __forceinline__ typename Frag<T>::type pack(const pa_f16v &a, int u)
+{
+    typename Frag<T>::type f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (T)a[8 * u + e];
+    return f;
+}
+
+// 16 bytes of a row from global memory, zeros when `ok` is false (the address is not touched then)
+__device__ __forceinline__ pa_u4 ldg16(const void *p, bool ok)
+{
+    pa_u4 z = {0, 0, 0, 0};
+    if (ok) z = *reinterpret_cast<const pa_u4 *>(p);
+    return z;
+}
+
+// fragment of a row held in global memory: elements 16 kk + 8 h .. of `row`, zeros past d (a multiple of 8)
+template <typename T> __device__ __forceinline__ typename Frag<T>::type ldrow(const T *row, int kk, int h, int d, bool ok)
+{
+    const int e0 = 16 * kk + 8 * h;
+    ok = ok && e0 < d;
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_bit_cast(typename Frag<T>::type, ldg16(row + e0, ok));
+    } else {
+        const pa_f4 a = __builtin_bit_cast(pa_f4, ldg16(row + e0, ok)), b = __builtin_bit_cast(pa_f4, ldg16(row + e0 + 4, ok));
+        return (pa_f8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+}
+
+// four floats as four elements of a row
+template <typename T> __device__ __forceinline__ void st4(T *p, float a, float b, float c, float d)
+{
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<t4 *>(p) = (t4){(T)a, (T)b, (T)c, (T)d};
+}
+
+// x / g for 0 <= x < 2^31 by one multiplication with m = ceil(2^32 / g): the excess x (m g - 2^32) / (g 2^32) is below 1/2, so the product is the
+// quotient or one more, and one comparison settles it
+struct Div {
+    u32 g, m;
+    __host__ __device__ Div() : g(1), m(0) {}
+    explicit __host__ Div(int d) : g((u32)d), m((u32)((0x100000000ull + (u32)d - 1) / (u32)d)) {}
+    __device__ __forceinline__ int div(int x) const
+    {
+        if (g == 1) return x;
+        u32 q = __umulhi((u32)x, m);
+        if (q * g > (u32)x) --q;
+        return (int)q;
+    }
+};
+
+// What a query sees.  Query i of sequence b stands at position p = start_b + i; key j is in view if j < len_b, j <= p + right, and j >= p - left or
+// j < sinks.  A query at p >= len_b is padding and sees nothing.  Both device values are clamped to the buffer, so that no value faults.
+struct View {
+    int m, left, right, sinks;
+    const int *start, *length;
+
+    __device__ __forceinline__ int len(int b) const { return length ? min(max(length[b], 0), m) : m; }
+    __device__ __forceinline__ int first(int b) const { return start ? min(max(start[b], 0), m) : 0; }
+};
+
+// keys in view of one row as [lo, lo + span] and [0, sink); nothing: lo out of reach
+struct Keys {
+    int lo, sink;
+    u32 span;
+    bool ok;
+
+    __device__ __forceinline__ Keys(const View &v, int p, int len, bool there)
+    {
+        ok = there && p < len;
+        const int hi = min(p + v.right, len - 1);
+        lo = ok ? max(p - v.left, 0) : NOWHERE;
+        span = ok ? (u32)(hi - lo) : 0u;
+        sink = ok ? min(v.sinks, hi + 1) : 0;
+    }
+    __device__ __forceinline__ bool sees(int j) const { return (u32)(j - lo) <= span || j < sink; }
+};
+
+// the KT-key tiles that rows at positions p0 .. p1 walk: nsk tiles of first tokens, then [lo, hi)
+template <int KT> struct TileList {
+    int nsk, lo, n;
+
+    __device__ __forceinline__ TileList(const View &v, int p0, int p1, int len)
+    {
+        nsk = lo = n = 0;
+        p1 = min(p1, len - 1);
+        if (p0 > p1) return;                                   // padding rows only
+        const int hi = min(p1 + v.right, len - 1) + 1;
+        lo = max(p0 - v.left, 0) / KT;
+        nsk = min((min(v.sinks, hi) + KT - 1) / KT, lo);
+        n = nsk + (hi + KT - 1) / KT - lo;
+    }
+    __device__ __forceinline__ int tile(int i) const { return i < nsk ? i : lo + i - nsk; }
+};
+
+static inline int width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }      // padded head width
+
+}  // namespace pa_attn
+
+// argument checks that forward and backward share
+static inline int window_attention_check(const char *name, int dtype, int b, int n, int m, int h, int hk, int d, int left, int right, int sinks, float scale)
+{
+    PA_REQUIRE(dtype >= PA_DT_F32 && dtype <= PA_DT_BF16, "%s: dtype %d is none of 0 (float32), 1 (float16), 2 (bfloat16)", name, dtype);
+    PA_REQUIRE(b >= 0 && n >= 0 && m >= 0 && n <= pa_attn::MAXLEN && m <= pa_attn::MAXLEN, "%s: bad sizes b=%d n=%d m=%d (up to 2^28 tokens)", name, b, n, m);
+    PA_REQUIRE(h > 0 && hk > 0 && h % hk == 0, "%s: %d query heads do not share %d key heads evenly", name, h, hk);
+    PA_REQUIRE((long)n * (h / hk) <= pa_attn::UNBOUNDED, "%s: n (h / hk) = %ld rows exceed 2^29", name, (long)n * (h / hk));
+    PA_REQUIRE(d > 0 && d <= 128 && d % 8 == 0, "%s: head width %d is not a multiple of 8 up to 128", name, d);
+    PA_REQUIRE(left >= -1 && right >= -1 && left <= pa_attn::MAXLEN && right <= pa_attn::MAXLEN && sinks >= 0, "%s: bad window left=%d right=%d sinks=%d", name, left,
+               right, sinks);
+    PA_REQUIRE(scale > 0.f && scale < INFINITY, "%s: the scale has to be positive and finite", name);
+    return PA_OK;
+}
+
+// element type and padded head width as template arguments of F: runs F(T, DT)
+#define PA_ATTN_WIDTH(T, d, F)                                                  \
+    do {                                                                        \
+        if ((d) <= 32) { F(T, 32); }                                            \
+        else if ((d) <= 64) { F(T, 64); }                                       \
+        else if ((d) <= 96) { F(T, 96); }                                       \
+        else { F(T, 128); }                                                     \
+    } while (0)
+#define PA_ATTN_DISPATCH(dtype, d, F)                                           \
+    do {                                                                        \
+        if ((dtype) == PA_DT_F32) PA_ATTN_WIDTH(float, d, F);                   \
+        else if ((dtype) == PA_DT_F16) PA_ATTN_WIDTH(_Float16, d, F);           \
+        else PA_ATTN_WIDTH(__bf16, d, F);                                       \
+    } while (0)

@@ -1,0 +1,258 @@
+// Attention with a sliding window and a few first tokens that stay in view, forward.
+//
+//     o_i = sum_j P_ij v_j,   P_ij = exp(s_ij) / sum_j exp(s_ij),   s_ij = scale q_i . k_j   over the keys j in view of row i (View, pa_attn.h)
+//
+// One pass over the keys with a running maximum and sum: O(window) work and nothing N x M in memory.  A workgroup owns 128 rows -- the N queries of
+// the G heads that share a key head, query-major, so that one tile of keys serves all of them -- and walks the 64-key tiles that its rows can see:
+// the tiles of the first tokens, then one contiguous range.  A wave owns 32 rows.  S^T = K Q^T puts one row into a lane's registers (maximum and
+// sum need one exchange between the two half waves), and the registers of P^T feed O^T += V^T P^T without leaving the lane; V is read transposed
+// from LDS.  K and V tiles are fetched one tile ahead into registers and stored to the other half of a double buffer, one barrier a tile.
+//
+// Roundings: s, maximum, sum and o are 32-bit; P is rounded to the type of V for the second product (16-bit types), with P <= 2^8 by the running
+// maximum, which is only moved when a row's maximum grows by more than 2^8 (the quotient is the same for any reference value).
+#include "pa_attn.h"
+
+using namespace pa_attn;
+
+namespace {
+
+constexpr int QT = 128, KT = 64;
+
+struct FwdArgs {
+    const void *q, *k, *v;
+    void *out;
+    float *lse, *part;
+    long qb, qn, qh, kb, kn, kh, vb, vn, vh;
+    int B, N, H, Hk, D, G, splits, nqt;
+    float c;                  // scale log2(e)
+    View view;
+    Div g;
+};
+
+template <typename T, int DT, bool SPLIT>
+__global__ __launch_bounds__(256) void fwd_kernel(const FwdArgs a)
+{
+    typedef Tile<T, DT> L;
+    typedef typename Frag<T>::type F;
+    constexpr int NF = KT * L::CH / 256;                       // chunks a thread stages per tensor
+    constexpr int TB = KT * L::RB;
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K tile, V tile]
+    const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
+
+    const int qt = blockIdx.x % a.nqt, bh = blockIdx.x / a.nqt, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int rows = a.N * a.G, len = a.view.len(b), start = a.view.first(b);
+    const int r0 = qt * QT;
+    const TileList<KT> tiles(a.view, start + a.g.div(r0), start + a.g.div(min(r0 + QT, rows) - 1), len);
+    int t0 = 0, t1 = tiles.n;
+    if (SPLIT) {
+        t0 = (int)((long)tiles.n * blockIdx.y / a.splits);
+        t1 = (int)((long)tiles.n * (blockIdx.y + 1) / a.splits);
+    }
+
+    // this lane's row
+    const int row = r0 + wave * 32 + (l & 31), i = a.g.div(min(row, rows - 1)), hq = hk * a.G + min(row, rows - 1) - i * a.G;
+    const Keys keys(a.view, start + i, len, row < rows);
+    F qf[DT / 16];
+    {
+        const T *qp = (const T *)a.q + b * a.qb + i * a.qn + hq * a.qh;
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk) qf[kk] = ldrow<T>(qp, kk, h, a.D, row < rows);
+    }
+    // the wave's rows: positions of the first and of the last one that is not padding
+    const int wr = __builtin_amdgcn_readfirstlane(r0 + wave * 32);
+    const int wp0 = start + a.g.div(min(wr, rows - 1)), wp1 = min(start + a.g.div(min(wr + 31, rows - 1)), len - 1);
+    const bool wave_on = wr < rows && wp0 < len;
+    const int wlo = max(wp0 - a.view.left, 0), whi = min(wp1 + a.view.right, len - 1);                  // some row sees [wlo, whi]
+    const int flo = max(wp1 - a.view.left, 0), fhi = min(wp0 + a.view.right, len - 1);                  // every row sees [flo, fhi]
+
+    const T *kp = (const T *)a.k + b * a.kb + hk * a.kh, *vp = (const T *)a.v + b * a.vb + hk * a.vh;
+    pa_u4 pk[NF], pv[NF];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < NF; ++u) {
+            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH, j = t * KT + r;
+            const bool ok = j < len && c * L::EC < a.D;        // rows behind the sequence are zeros: what they hold never meets a product
+            pk[u] = ldg16(kp + (long)j * a.kn + c * L::EC, ok);
+            pv[u] = ldg16(vp + (long)j * a.vn + c * L::EC, ok);
+        }
+    };
+
+    pa_f16v o[DT / 32];
+#pragma unroll
+    for (int ct = 0; ct < DT / 32; ++ct) o[ct] = (pa_f16v)(0.f);
+    float m_run = -INFINITY, l_run = 0.f;
+
+    if (t0 < t1) fetch(tiles.tile(t0));
+    for (int it = t0; it < t1; ++it) {
+        char *ks = smem + ((it - t0) & 1) * 2 * TB, *vs = ks + TB;
+#pragma unroll
+        for (int u = 0; u < NF; ++u) {
+            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH;
+            *reinterpret_cast<pa_u4 *>(ks + L::at(r, c)) = pk[u];
+            *reinterpret_cast<pa_u4 *>(vs + L::at(r, c)) = pv[u];
+        }
+        __syncthreads();                                       // the previous tile's readers of this half passed the barrier before this one
+        const int j0 = tiles.tile(it) * KT;
+        if (it + 1 < t1) fetch(tiles.tile(it + 1));
+        if (!wave_on) continue;
+#pragma unroll
+        for (int sub = 0; sub < KT / 32; ++sub) {
+            const int js = j0 + sub * 32;
+            if (!((js <= whi && js + 31 >= wlo) || js < min(a.view.sinks, whi + 1))) continue;
+            pa_f16v s = (pa_f16v)(0.f);
+#pragma unroll
+            for (int kk = 0; kk < DT / 16; ++kk) mma(s, L::ld(ks, sub * 32, kk), qf[kk]);
+            if (!(js >= flo && js + 31 <= fhi)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = keys.sees(js + 8 * (r >> 2) + 4 * h + (r & 3)) ? s[r] : -INFINITY;
+            }
+            float mt = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
+            mt = fmaxf(mt, other_half(mt)) * a.c;
+            if (__any(mt > m_run + 8.f)) {                     // -inf + 8 = -inf: the first visible key of a row always moves it
+                const float mn = fmaxf(m_run, mt), sc = mn > -INFINITY ? ex2(m_run - mn) : 0.f;
+#pragma unroll
+                for (int ct = 0; ct < DT / 32; ++ct)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[ct][r] *= sc;
+                l_run *= sc;
+                m_run = mn;
+            }
+            const float mref = m_run > -INFINITY ? m_run : 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = ex2(__builtin_fmaf(s[r], a.c, -mref));
+                l_run += s[r];
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const F p = pack<T>(s, u);
+#pragma unroll
+                for (int ct = 0; ct < DT / 32; ++ct) mma(o[ct], L::ldt(vs, sub * 32 + 16 * u, ct * 32), p);
+            }
+        }
+    }
+
+    l_run += other_half(l_run);
+    if (row >= rows) return;
+    if (SPLIT) {
+        const size_t all = (size_t)a.B * a.Hk * rows, at = (size_t)blockIdx.y * all + (size_t)bh * rows + row;
+        float *po = a.part + at * DT, *pm = a.part + (size_t)a.splits * all * DT + at * 2;
+#pragma unroll
+        for (int ct = 0; ct < DT / 32; ++ct)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                *reinterpret_cast<pa_f4 *>(po + ct * 32 + 8 * u + 4 * h) = (pa_f4){o[ct][4 * u], o[ct][4 * u + 1], o[ct][4 * u + 2], o[ct][4 * u + 3]};
+        if (h == 0) {
+            pm[0] = m_run;
+            pm[1] = l_run;
+        }
+        return;
+    }
+    const float inv = keys.ok && l_run != 0.f ? 1.0f / l_run : 0.f;         // padding rows computed on zeros: their output is 0
+    T *op = (T *)a.out + (((size_t)b * a.N + i) * a.H + hq) * a.D;
+#pragma unroll
+    for (int ct = 0; ct < DT / 32; ++ct)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = ct * 32 + 8 * u + 4 * h;
+            if (c < a.D) st4<T>(op + c, o[ct][4 * u] * inv, o[ct][4 * u + 1] * inv, o[ct][4 * u + 2] * inv, o[ct][4 * u + 3] * inv);
+        }
+    if (a.lse && h == 0) a.lse[((size_t)b * a.H + hq) * a.N + i] = inv == 0.f ? INFINITY : m_run + __builtin_amdgcn_logf(l_run);
+}
+
+// The rows of a split launch: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  A thread owns four elements of a row.
+template <typename T, int DT>
+__global__ __launch_bounds__(256) void join_kernel(const FwdArgs a)
+{
+    constexpr int TR = DT / 4;
+    const int rows = a.N * a.G;
+    const size_t all = (size_t)a.B * a.Hk * rows;
+    const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) / TR;
+    const int c = (int)(((size_t)blockIdx.x * 256 + threadIdx.x) % TR) * 4;
+    if (at >= all) return;
+    const float *pm = a.part + (size_t)a.splits * all * DT;
+    float m = -INFINITY, l = 0.f;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, pm[(s * all + at) * 2]);
+    const float mref = m > -INFINITY ? m : 0.f;
+    pa_f4 o = (pa_f4)(0.f);
+    for (int s = 0; s < a.splits; ++s) {
+        const float w = ex2(pm[(s * all + at) * 2] - mref);
+        l += w * pm[(s * all + at) * 2 + 1];
+        o += w * *reinterpret_cast<const pa_f4 *>(a.part + (s * all + at) * DT + c);
+    }
+    const int bh = (int)(at / rows), row = (int)(at - (size_t)bh * rows), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int i = a.g.div(row), hq = hk * a.G + row - i * a.G;
+    const float inv = a.view.first(b) + i < a.view.len(b) && l != 0.f ? 1.0f / l : 0.f;
+    if (c < a.D) st4<T>((T *)a.out + (((size_t)b * a.N + i) * a.H + hq) * a.D + c, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (a.lse && c == 0) a.lse[((size_t)b * a.H + hq) * a.N + i] = inv == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// Work is split over the keys when the rows alone leave the chip idle: fewer than 256 workgroups (one per CU).  Two per CU are aimed at, each with
+// at least four tiles, because a part costs one round trip of its rows in 32 bits.
+int fwd_splits(int B, int N, int M, int H, int Hk, int left, int right, int sinks)
+{
+    const long G = H / Hk, wgs = (long)B * Hk * pa_div_up((long)N * G, QT);
+    if (wgs >= 256) return 1;
+    const long span = (long)left + right + QT / G + 1;                       // longest range of keys of one workgroup
+    const long tiles = pa_div_up(M < span ? M : span, KT) + (left < M ? pa_div_up(sinks, KT) : 0);
+    const long want = 512 / wgs, most = tiles / 4;
+    const long s = want < most ? want : most;
+    return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
+}
+
+template <typename T, int DT>
+int launch_fwd(const FwdArgs &a, hipStream_t st)
+{
+    constexpr int lds = 4 * KT * DT * (int)sizeof(T);
+    const dim3 grid((unsigned)((long)a.nqt * a.B * a.Hk), (unsigned)a.splits);
+    if (a.splits > 1) {
+        if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&fwd_kernel<T, DT, true>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        hipLaunchKernelGGL((fwd_kernel<T, DT, true>), grid, dim3(256), lds, st, a);
+        const long threads = (long)a.B * a.Hk * a.N * a.G * (DT / 4);
+        hipLaunchKernelGGL((join_kernel<T, DT>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+    } else {
+        if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&fwd_kernel<T, DT, false>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        hipLaunchKernelGGL((fwd_kernel<T, DT, false>), grid, dim3(256), lds, st, a);
+    }
+    return 0;
+}
+
+}  // namespace
+
+PA_API long pa_window_attention_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks)
+{
+    if (b <= 0 || n <= 0 || h <= 0 || hk <= 0 || h % hk != 0) return 0;
+    const int l = left < 0 ? UNBOUNDED : left, r = right < 0 ? UNBOUNDED : right;
+    const int s = fwd_splits(b, n, m, h, hk, l, r, sinks);
+    return s <= 1 ? 0 : (long)s * b * n * h * (width(d) + 2);
+}
+
+PA_API int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn,
+                               long kh, const void *v, long vb, long vn, long vh, int left, int right, int sinks, float scale, const int *start,
+                               const int *length, void *out, float *lse, float *scratch, pa_stream_t stream)
+{
+    int rc = window_attention_check("pa_window_attention", dtype, b, n, m, h, hk, d, left, right, sinks, scale);
+    if (rc != PA_OK) return rc;
+    if (b == 0 || n == 0) return PA_OK;
+    PA_REQUIRE(q && out && (m == 0 || (k && v)), "pa_window_attention: null tensor");
+    FwdArgs a;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.part = scratch;
+    a.qb = qb; a.qn = qn; a.qh = qh; a.kb = kb; a.kn = kn; a.kh = kh; a.vb = vb; a.vn = vn; a.vh = vh;
+    a.B = b; a.N = n; a.H = h; a.Hk = hk; a.D = d; a.G = h / hk;
+    a.view.m = m; a.view.left = left < 0 ? UNBOUNDED : left; a.view.right = right < 0 ? UNBOUNDED : right; a.view.sinks = sinks < m ? sinks : m;
+    a.view.start = start; a.view.length = length;
+    a.c = scale * 1.4426950408889634f;
+    a.g = Div(a.G);
+    a.nqt = pa_div_up((long)n * a.G, QT);
+    a.splits = fwd_splits(b, n, m, h, hk, a.view.left, a.view.right, sinks);
+    PA_REQUIRE((long)a.nqt * b * hk < (1l << 31), "pa_window_attention: too many workgroups");
+    PA_REQUIRE(a.splits == 1 || scratch, "pa_window_attention: this size needs pa_window_attention_scratch_floats() of scratch");
+    hipStream_t st = (hipStream_t)stream;
+#define FWD(T, DT) launch_fwd<T, DT>(a, st)
+    PA_ATTN_DISPATCH(dtype, d, FWD);
+#undef FWD
+    PA_CHECK_LAUNCH("pa_window_attention");
+    return PA_OK;
+}

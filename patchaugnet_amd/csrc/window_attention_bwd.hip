@@ -1,0 +1,429 @@
+// Gradients of the attention with a sliding window and first tokens that stay in view (window_attention.hip).
+//
+//     P_ij = exp(s_ij - lse_i)            delta_i = do_i . o_i            dS_ij = P_ij (do_i . v_j - delta_i)
+//     dq_i = scale sum_j dS_ij k_j        dk_j = scale sum_i dS_ij q_i        dv_j = sum_i P_ij do_i       (i over all rows that share key head)
+//
+// Two kernels recompute the scores from q, k and the forward's lse (log2 units): one owns rows and walks keys (dq, and delta, which it leaves for the
+// other), one owns keys and walks rows (dk, dv).  That is 7 products where one kernel with both would need 5, but every gradient is summed by one
+// owner in a fixed order: no atomics, the same bits every run.  The registers of P and dS feed the second products as they are (pa_attn.h); q, do
+// and k are read from LDS both as rows and transposed.
+//
+// The keys of the first tokens are seen by every later row, so their walk is N / window times longer than any other's: it is cut into slices that
+// write 32-bit partial sums, joined by a second launch; so are all walks when the keys alone do not fill the chip.
+//
+// Roundings: P and dS are rounded to the operand type for the second products (16-bit types); the scale is applied to the 32-bit sums, so that dS is
+// rounded before it gets smaller.
+#include "pa_attn.h"
+
+using namespace pa_attn;
+
+namespace {
+
+constexpr int QT = 128, KT = 64;       // dq: rows of a workgroup, keys of a tile
+constexpr int KB = 128, RT = 64;       // dk, dv: keys of a workgroup, rows of a tile
+
+struct BwdArgs {
+    const void *q, *k, *v, *out, *dout;
+    const float *lse;
+    float *delta, *part;
+    void *dq, *dk, *dv;
+    long qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh;
+    int B, N, H, Hk, D, G, nqt;
+    int nst, nkt, ssink, snorm;        // key tiles with first tokens, all key tiles, slices of either kind
+    float c, scale;
+    View view;
+    Div g;
+};
+
+template <typename T, int DT>
+__global__ __launch_bounds__(256) void dq_kernel(const BwdArgs a)
+{
+    typedef Tile<T, DT> L;
+    typedef typename Frag<T>::type F;
+    constexpr int NF = KT * L::CH / 256, TB = KT * L::RB;
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K tile, V tile]
+    const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
+    const int qt = blockIdx.x % a.nqt, bh = blockIdx.x / a.nqt, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int rows = a.N * a.G, len = a.view.len(b), start = a.view.first(b);
+    const int r0 = qt * QT;
+
+    const int row = r0 + wave * 32 + (l & 31), i = a.g.div(min(row, rows - 1)), hq = hk * a.G + min(row, rows - 1) - i * a.G;
+    const Keys keys(a.view, start + i, len, row < rows);
+    const size_t at = ((size_t)b * a.H + hq) * a.N + i;
+    F qf[DT / 16], gf[DT / 16];
+    float delta = 0.f;
+    {
+        const T *qp = (const T *)a.q + b * a.qb + i * a.qn + hq * a.qh, *gp = (const T *)a.dout + b * a.gb + i * a.gn + hq * a.gh;
+        const T *op = (const T *)a.out + (((size_t)b * a.N + i) * a.H + hq) * a.D;
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk) {
+            qf[kk] = ldrow<T>(qp, kk, h, a.D, keys.ok);
+            gf[kk] = ldrow<T>(gp, kk, h, a.D, keys.ok);
+            const F of = ldrow<T>(op, kk, h, a.D, keys.ok);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)gf[kk][e], (float)of[e], delta);
+        }
+        delta += other_half(delta);
+    }
+    const float lse = keys.ok ? a.lse[at] : INFINITY;
+    if (h == 0 && row < rows) a.delta[at] = delta;
+
+    const int wr = __builtin_amdgcn_readfirstlane(r0 + wave * 32);
+    const int wp0 = start + a.g.div(min(wr, rows - 1)), wp1 = min(start + a.g.div(min(wr + 31, rows - 1)), len - 1);
+    const bool wave_on = wr < rows && wp0 < len;
+    const int wlo = max(wp0 - a.view.left, 0), whi = min(wp1 + a.view.right, len - 1);
+    const int flo = max(wp1 - a.view.left, 0), fhi = min(wp0 + a.view.right, len - 1);
+
+    const T *kp = (const T *)a.k + b * a.kb + hk * a.kh, *vp = (const T *)a.v + b * a.vb + hk * a.vh;
+    pa_u4 pk[NF], pv[NF];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < NF; ++u) {
+            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH, j = t * KT + r;
+            const bool ok = j < len && c * L::EC < a.D;
+            pk[u] = ldg16(kp + (long)j * a.kn + c * L::EC, ok);
+            pv[u] = ldg16(vp + (long)j * a.vn + c * L::EC, ok);
+        }
+    };
+
+    pa_f16v dq[DT / 32];
+#pragma unroll
+    for (int ct = 0; ct < DT / 32; ++ct) dq[ct] = (pa_f16v)(0.f);
+
+    const TileList<KT> tiles(a.view, start + a.g.div(r0), start + a.g.div(min(r0 + QT, rows) - 1), len);
+    if (tiles.n) fetch(tiles.tile(0));
+    for (int it = 0; it < tiles.n; ++it) {
+        char *ks = smem + (it & 1) * 2 * TB, *vs = ks + TB;
+#pragma unroll
+        for (int u = 0; u < NF; ++u) {
+            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH;
+            *reinterpret_cast<pa_u4 *>(ks + L::at(r, c)) = pk[u];
+            *reinterpret_cast<pa_u4 *>(vs + L::at(r, c)) = pv[u];
+        }
+        __syncthreads();
+        const int j0 = tiles.tile(it) * KT;
+        if (it + 1 < tiles.n) fetch(tiles.tile(it + 1));
+        if (!wave_on) continue;
+#pragma unroll
+        for (int sub = 0; sub < KT / 32; ++sub) {
+            const int js = j0 + sub * 32;
+            if (!((js <= whi && js + 31 >= wlo) || js < min(a.view.sinks, whi + 1))) continue;
+            pa_f16v s = (pa_f16v)(0.f), dp = (pa_f16v)(0.f);
+#pragma unroll
+            for (int kk = 0; kk < DT / 16; ++kk) {
+                mma(s, L::ld(ks, sub * 32, kk), qf[kk]);
+                mma(dp, L::ld(vs, sub * 32, kk), gf[kk]);
+            }
+            if (!(js >= flo && js + 31 <= fhi)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = keys.sees(js + 8 * (r >> 2) + 4 * h + (r & 3)) ? s[r] : -INFINITY;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = ex2(__builtin_fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const F ds = pack<T>(s, u);
+#pragma unroll
+                for (int ct = 0; ct < DT / 32; ++ct) mma(dq[ct], L::ldt(ks, sub * 32 + 16 * u, ct * 32), ds);
+            }
+        }
+    }
+    if (row >= rows) return;
+    T *dp = (T *)a.dq + (((size_t)b * a.N + i) * a.H + hq) * a.D;
+    const float f = keys.ok ? a.scale : 0.f;
+#pragma unroll
+    for (int ct = 0; ct < DT / 32; ++ct)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = ct * 32 + 8 * u + 4 * h;
+            if (c < a.D) st4<T>(dp + c, dq[ct][4 * u] * f, dq[ct][4 * u + 1] * f, dq[ct][4 * u + 2] * f, dq[ct][4 * u + 3] * f);
+        }
+}
+
+// what a workgroup of the dk, dv launch owns: the slices of the first tokens' tiles come first (they are the longest walks)
+struct KeyTile {
+    int bh, tile, slice, slices;
+    long slot;                          // place of its partial sums; < 0: it writes the gradients itself
+
+    __device__ __forceinline__ KeyTile(const BwdArgs &a, long id)
+    {
+        const long nsink = (long)a.B * a.Hk * a.nst * a.ssink;
+        if (id < nsink) {
+            slices = a.ssink;
+            slot = slices > 1 ? id : -1;
+            slice = (int)(id % slices);
+            id /= slices;
+            tile = (int)(id % a.nst);
+            bh = (int)(id / a.nst);
+        } else {
+            id -= nsink;
+            slices = a.snorm;
+            slot = slices > 1 ? (a.ssink > 1 ? nsink : 0) + id : -1;
+            slice = (int)(id % slices);
+            id /= slices;
+            tile = a.nst + (int)(id % (a.nkt - a.nst));
+            bh = (int)(id / (a.nkt - a.nst));
+        }
+    }
+};
+
+template <typename T, int DT>
+__global__ __launch_bounds__(256) void dkv_kernel(const BwdArgs a)
+{
+    typedef Tile<T, DT> L;
+    typedef typename Frag<T>::type F;
+    constexpr int NF = RT * L::CH / 256, TB = RT * L::RB, BUF = 2 * TB + 3 * RT * 4;
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][Q tile, dO tile, lse, delta, position]
+    const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
+    const KeyTile kt(a, blockIdx.x);
+    const int b = kt.bh / a.Hk, hk = kt.bh - b * a.Hk;
+    const int len = a.view.len(b), start = a.view.first(b);
+    const int k0 = kt.tile * KB, k1 = min(k0 + KB, len) - 1;
+
+    // rows that see any of these keys: positions k0 - right .. k1 + left, or to the end where first tokens are among the keys
+    int ra = 0, rb = 0;
+    if (k0 <= k1) {
+        const int last = min(a.N - 1, len - 1 - start), ia = max(k0 - a.view.right - start, 0);
+        const int ib = k0 < a.view.sinks ? last : min(last, k1 + a.view.left - start);
+        if (ia <= ib) {
+            ra = ia * a.G;
+            rb = (ib + 1) * a.G;
+        }
+    }
+    const int all = (rb - ra + RT - 1) / RT;
+    const int t0 = (int)((long)all * kt.slice / kt.slices), t1 = (int)((long)all * (kt.slice + 1) / kt.slices);
+
+    const int wk = __builtin_amdgcn_readfirstlane(k0 + wave * 32), wk1 = min(wk + 31, len - 1);
+    const bool wave_on = wk < len;
+    const int j = wk + (l & 31);
+    // this lane's key is seen from positions plo .. plo + span
+    const int plo = j < len ? j - a.view.right : NOWHERE;
+    const u32 span = j >= len ? 0u : j < a.view.sinks ? 0x7fffffffu : (u32)a.view.left + (u32)a.view.right;
+    F kf[DT / 16], vf[DT / 16];
+    {
+        const T *kp = (const T *)a.k + b * a.kb + hk * a.kh + (long)j * a.kn, *vp = (const T *)a.v + b * a.vb + hk * a.vh + (long)j * a.vn;
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk) {
+            kf[kk] = ldrow<T>(kp, kk, h, a.D, j < len);
+            vf[kk] = ldrow<T>(vp, kk, h, a.D, j < len);
+        }
+    }
+
+    pa_u4 pq[NF], pg[NF];
+    float pl = 0.f, pd = 0.f;
+    int pp = 0;
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < NF; ++u) {
+            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH, row = ra + t * RT + r;
+            const int i = a.g.div(min(row, rb - 1)), hq = hk * a.G + row - i * a.G;
+            const bool ok = row < rb && c * L::EC < a.D;       // padding rows are behind rb
+            pq[u] = ldg16((const T *)a.q + b * a.qb + i * a.qn + hq * a.qh + c * L::EC, ok);
+            pg[u] = ldg16((const T *)a.dout + b * a.gb + i * a.gn + hq * a.gh + c * L::EC, ok);
+        }
+        if (tid < RT) {
+            const int row = ra + t * RT + tid, i = a.g.div(min(row, rb - 1)), hq = hk * a.G + row - i * a.G;
+            const size_t at = ((size_t)b * a.H + hq) * a.N + i;
+            pl = row < rb ? a.lse[at] : INFINITY;
+            pd = row < rb ? a.delta[at] : 0.f;
+            pp = start + i;
+        }
+    };
+
+    pa_f16v dk[DT / 32], dv[DT / 32];
+#pragma unroll
+    for (int ct = 0; ct < DT / 32; ++ct) dk[ct] = dv[ct] = (pa_f16v)(0.f);
+
+    if (t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+        char *qs = smem + ((t - t0) & 1) * BUF, *gs = qs + TB;
+        float *ls = reinterpret_cast<float *>(gs + TB), *ds = ls + RT;
+        int *ps = reinterpret_cast<int *>(ds + RT);
+#pragma unroll
+        for (int u = 0; u < NF; ++u) {
+            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH;
+            *reinterpret_cast<pa_u4 *>(qs + L::at(r, c)) = pq[u];
+            *reinterpret_cast<pa_u4 *>(gs + L::at(r, c)) = pg[u];
+        }
+        if (tid < RT) {
+            ls[tid] = pl;
+            ds[tid] = pd;
+            ps[tid] = pp;
+        }
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        if (!wave_on) continue;
+#pragma unroll
+        for (int sub = 0; sub < RT / 32; ++sub) {
+            const int rs = ra + t * RT + sub * 32;
+            if (rs >= rb) continue;
+            const int p0 = start + a.g.div(rs), p1 = start + a.g.div(min(rs + 31, rb - 1));
+            if (!(p1 >= wk - a.view.right && (p0 <= wk1 + a.view.left || wk < a.view.sinks))) continue;
+            pa_f16v s = (pa_f16v)(0.f), dp = (pa_f16v)(0.f);
+#pragma unroll
+            for (int kk = 0; kk < DT / 16; ++kk) {
+                mma(s, L::ld(qs, sub * 32, kk), kf[kk]);
+                mma(dp, L::ld(gs, sub * 32, kk), vf[kk]);
+            }
+            const bool full = p0 >= wk + 31 - a.view.right && p1 <= wk + a.view.left && wk + 31 < len;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int rr = sub * 32 + 8 * u + 4 * h;
+                const pa_f4 lse = *reinterpret_cast<const pa_f4 *>(ls + rr), delta = *reinterpret_cast<const pa_f4 *>(ds + rr);
+                const int4 pos = *reinterpret_cast<const int4 *>(ps + rr);
+                const int pe[4] = {pos.x, pos.y, pos.z, pos.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * u + e;
+                    const float p = ex2(__builtin_fmaf(s[r], a.c, -lse[e]));
+                    s[r] = full || (u32)pe[e] - (u32)plo <= span ? p : 0.f;
+                    dp[r] = s[r] * (dp[r] - delta[e]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const F pf = pack<T>(s, u), df = pack<T>(dp, u);
+#pragma unroll
+                for (int ct = 0; ct < DT / 32; ++ct) {
+                    mma(dv[ct], L::ldt(gs, sub * 32 + 16 * u, ct * 32), pf);
+                    mma(dk[ct], L::ldt(qs, sub * 32 + 16 * u, ct * 32), df);
+                }
+            }
+        }
+    }
+    if (kt.slot >= 0) {
+        float *po = a.part + ((size_t)kt.slot * KB + wave * 32 + (l & 31)) * (2 * DT);
+#pragma unroll
+        for (int ct = 0; ct < DT / 32; ++ct)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int c = ct * 32 + 8 * u + 4 * h;
+                *reinterpret_cast<pa_f4 *>(po + c) = (pa_f4){dk[ct][4 * u], dk[ct][4 * u + 1], dk[ct][4 * u + 2], dk[ct][4 * u + 3]};
+                *reinterpret_cast<pa_f4 *>(po + DT + c) = (pa_f4){dv[ct][4 * u], dv[ct][4 * u + 1], dv[ct][4 * u + 2], dv[ct][4 * u + 3]};
+            }
+        return;
+    }
+    if (j >= a.view.m) return;
+    const size_t at = (((size_t)b * a.view.m + j) * a.Hk + hk) * a.D;
+    T *ko = (T *)a.dk + at, *vo = (T *)a.dv + at;
+    const float f = a.scale;
+#pragma unroll
+    for (int ct = 0; ct < DT / 32; ++ct)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = ct * 32 + 8 * u + 4 * h;
+            if (c < a.D) {
+                st4<T>(ko + c, dk[ct][4 * u] * f, dk[ct][4 * u + 1] * f, dk[ct][4 * u + 2] * f, dk[ct][4 * u + 3] * f);
+                st4<T>(vo + c, dv[ct][4 * u], dv[ct][4 * u + 1], dv[ct][4 * u + 2], dv[ct][4 * u + 3]);
+            }
+        }
+}
+
+// dk, dv of the sliced key tiles: the slices' partial sums in their order.  One workgroup per tile and 16 keys.
+template <typename T, int DT>
+__global__ __launch_bounds__(256) void dkv_join_kernel(const BwdArgs a, int first, int tiles, int slices, long slot0)
+{
+    constexpr int C = DT / 2;                                  // threads of a key: dk and dv, four elements each
+    const long id = ((long)blockIdx.x * 256 + threadIdx.x) / C;
+    const int c = (int)(((long)blockIdx.x * 256 + threadIdx.x) % C) * 4;
+    const long tile = id / KB;
+    const int r = (int)(id % KB);
+    if (tile >= (long)a.B * a.Hk * tiles) return;
+    const int bh = (int)(tile / tiles), t = first + (int)(tile % tiles), b = bh / a.Hk, hk = bh - b * a.Hk, j = t * KB + r;
+    if (j >= a.view.m) return;
+    const float *p = a.part + ((size_t)(slot0 + tile * slices) * KB + r) * (2 * DT) + c;
+    pa_f4 s = (pa_f4)(0.f);
+    for (int i = 0; i < slices; ++i) s += *reinterpret_cast<const pa_f4 *>(p + (size_t)i * KB * 2 * DT);
+    const size_t at = (((size_t)b * a.view.m + j) * a.Hk + hk) * a.D;
+    if (c < DT) {
+        if (c < a.D) st4<T>((T *)a.dk + at + c, s[0] * a.scale, s[1] * a.scale, s[2] * a.scale, s[3] * a.scale);
+    } else if (c - DT < a.D) {
+        st4<T>((T *)a.dv + at + c - DT, s[0], s[1], s[2], s[3]);
+    }
+}
+
+struct Slices {
+    int nst, nkt, ssink, snorm;
+};
+
+// Slices of a key tile's walk.  Keys that do not fill the chip (fewer than 512 workgroups) have their walks cut, each slice with at least four row
+// tiles; the tiles of first tokens are cut into as many slices as make theirs no longer than the others'.
+Slices slices_of(int B, int N, int M, int H, int Hk, int left, int right, int sinks)
+{
+    Slices s;
+    const long G = H / Hk;
+    s.nkt = pa_div_up(M, KB);
+    const long sk = sinks < M ? sinks : M;
+    s.nst = pa_div_up(sk, KB);
+    const long wgs = (long)B * Hk * s.nkt, reach = (long)left + right + KB, walk = pa_div_up((N < reach ? N : reach) * G, RT), whole = pa_div_up(N * G, RT);
+    long n = wgs ? 512 / wgs : 1;
+    if (n > walk / 4) n = walk / 4;
+    s.snorm = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+    long per = pa_div_up(walk, s.snorm);                        // row tiles of one slice
+    if (per < 4) per = 4;
+    long m = pa_div_up(whole, per);
+    s.ssink = s.nst == 0 || m < 1 ? 1 : m > 256 ? 256 : (int)m;
+    return s;
+}
+
+template <typename T, int DT>
+int launch_bwd(const BwdArgs &a, hipStream_t st)
+{
+    constexpr int lq = 4 * KT * DT * (int)sizeof(T), lk = 2 * (2 * RT * DT * (int)sizeof(T) + 3 * RT * 4);
+    if (lq > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&dq_kernel<T, DT>), hipFuncAttributeMaxDynamicSharedMemorySize, lq);
+    if (lk > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&dkv_kernel<T, DT>), hipFuncAttributeMaxDynamicSharedMemorySize, lk);
+    if (a.nqt) hipLaunchKernelGGL((dq_kernel<T, DT>), dim3((unsigned)((long)a.nqt * a.B * a.Hk)), dim3(256), lq, st, a);
+    const long bh = (long)a.B * a.Hk, sink = bh * a.nst * a.ssink, norm = bh * (a.nkt - a.nst) * a.snorm;
+    if (sink + norm == 0) return 0;
+    hipLaunchKernelGGL((dkv_kernel<T, DT>), dim3((unsigned)(sink + norm)), dim3(256), lk, st, a);
+    if (a.ssink > 1 && a.nst > 0)
+        hipLaunchKernelGGL((dkv_join_kernel<T, DT>), dim3((unsigned)(bh * a.nst * KB * (DT / 2) / 256)), dim3(256), 0, st, a, 0, a.nst, a.ssink, 0l);
+    if (a.snorm > 1 && a.nkt > a.nst)
+        hipLaunchKernelGGL((dkv_join_kernel<T, DT>), dim3((unsigned)(bh * (a.nkt - a.nst) * KB * (DT / 2) / 256)), dim3(256), 0, st, a, a.nst, a.nkt - a.nst, a.snorm,
+                           a.ssink > 1 ? sink : 0l);
+    return 0;
+}
+
+}  // namespace
+
+// floats of scratch: delta (B H N), then the partial sums of sliced walks
+PA_API long pa_window_attention_backward_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks)
+{
+    if (b <= 0 || n <= 0 || h <= 0 || hk <= 0 || h % hk != 0 || m < 0 || sinks < 0) return 0;
+    const Slices s = slices_of(b, n, m, h, hk, left < 0 ? UNBOUNDED : left, right < 0 ? UNBOUNDED : right, sinks);
+    const long bh = (long)b * hk, slots = (s.ssink > 1 ? bh * s.nst * s.ssink : 0) + (s.snorm > 1 ? bh * (s.nkt - s.nst) * s.snorm : 0);
+    return pa_div_up((long)b * h * n, 4) * 4l + slots * KB * 2 * width(d);
+}
+
+PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb,
+                                        long kn, long kh, const void *v, long vb, long vn, long vh, const void *out, const float *lse, const void *dout, long gb,
+                                        long gn, long gh, int left, int right, int sinks, float scale, const int *start, const int *length, void *dq, void *dk,
+                                        void *dv, float *scratch, pa_stream_t stream)
+{
+    int rc = window_attention_check("pa_window_attention_backward", dtype, b, n, m, h, hk, d, left, right, sinks, scale);
+    if (rc != PA_OK) return rc;
+    if (b == 0 || (n == 0 && m == 0)) return PA_OK;
+    PA_REQUIRE((n == 0 || (q && out && lse && dout && dq && scratch)) && (m == 0 || (k && v && dk && dv)), "pa_window_attention_backward: null tensor");
+    BwdArgs a;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.dout = dout; a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv;
+    a.delta = scratch;
+    a.part = scratch + pa_div_up((long)b * h * n, 4) * 4l;
+    a.qb = qb; a.qn = qn; a.qh = qh; a.kb = kb; a.kn = kn; a.kh = kh; a.vb = vb; a.vn = vn; a.vh = vh; a.gb = gb; a.gn = gn; a.gh = gh;
+    a.B = b; a.N = n; a.H = h; a.Hk = hk; a.D = d; a.G = h / hk;
+    a.view.m = m; a.view.left = left < 0 ? UNBOUNDED : left; a.view.right = right < 0 ? UNBOUNDED : right; a.view.sinks = sinks < m ? sinks : m;
+    a.view.start = start; a.view.length = length;
+    a.scale = scale;
+    a.c = scale * 1.4426950408889634f;
+    a.g = Div(a.G);
+    a.nqt = pa_div_up((long)n * a.G, QT);
+    const Slices s = slices_of(b, n, m, h, hk, a.view.left, a.view.right, sinks);
+    a.nst = s.nst; a.nkt = s.nkt; a.ssink = s.ssink; a.snorm = s.snorm;
+    PA_REQUIRE((long)a.nqt * b * hk < (1l << 31) && (long)b * hk * ((long)s.nst * s.ssink + (long)(s.nkt - s.nst) * s.snorm) * 32 < (1l << 31),
+               "pa_window_attention_backward: too many workgroups");
+    hipStream_t st = (hipStream_t)stream;
+#define BWD(T, DT) launch_bwd<T, DT>(a, st)
+    PA_ATTN_DISPATCH(dtype, d, BWD);
+#undef BWD
+    PA_CHECK_LAUNCH("pa_window_attention_backward");
+    return PA_OK;
+}

@@ -1,0 +1,240 @@
+"""attention.window_attention (csrc/window_attention.hip, window_attention_bwd.hip) against its 64-bit statement, forward and gradients."""
+import pytest
+import torch
+
+from _attention_ref import close, reference
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _qkv(B, N, M, H, Hk, D, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(s, generator=g, device="cuda").to(dtype) for s in ((B, N, H, D), (B, M, Hk, D), (B, M, Hk, D), (B, N, H, D))]
+
+
+def _ints(v):
+    return None if v is None else torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _run(q, k, v, do, left, right, sinks, lengths=None, starts=None, scale=None):
+    from patchaugnet_amd.attention import window_attention
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = window_attention(*leaves, left=left, right=right, sinks=sinks, scale=scale, lengths=_ints(lengths), q_start=_ints(starts))
+    grads = torch.autograd.grad(out, leaves, do)
+    return dict(zip(("out", "dq", "dk", "dv"), (out.detach(),) + grads))
+
+
+def _check(q, k, v, do, left, right, sinks, lengths=None, starts=None, scale=None):
+    got = _run(q, k, v, do, left, right, sinks, lengths, starts, scale)
+    val, tol = reference(q, k, v, left, right, sinks, scale, lengths, starts, do)
+    for n in val:
+        assert got[n].dtype == q.dtype
+        close(got[n], val[n], tol[n], n)
+    return got
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [8, 32, 40, 64, 72, 96, 128])
+def test_head_widths(dtype, D):
+    _check(*_qkv(2, 150, 150, 4, 2, D, dtype, seed=D), 37, 0, 3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,left,right,sinks", [
+    (1, None, 0, 0), (1, 0, 0, 0), (2, 0, 0, 1), (31, 5, 5, 0), (33, None, None, 0), (64, 63, 0, 0), (65, 64, 0, 64), (127, 0, 0, 0), (129, 0, 127, 2),
+    (200, None, 0, 5), (257, 1, 1, 70), (300, 31, 33, 129), (300, 1000, 1000, 7), (513, 128, 0, 300)])
+def test_lengths_and_windows(dtype, N, left, right, sinks):
+    _check(*_qkv(1, N, N, 2, 1, 32, dtype, seed=N), left, right, sinks)
+
+
+@pytest.mark.parametrize("H,Hk", [(1, 1), (3, 3), (3, 1), (6, 2), (8, 1), (40, 1), (7, 7)])
+def test_shared_heads(H, Hk):
+    _check(*_qkv(2, 70, 70, H, Hk, 16, F16, seed=H), 20, 0, 4)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_padded_batch(dtype):
+    lengths = [130, 0, 1, 64, 77, 200, -3]
+    q, k, v, do = _qkv(7, 130, 130, 2, 2, 24, dtype)
+    got = _check(q, k, v, do, 17, 9, 2, lengths)
+    for b, n in enumerate(lengths):
+        n = min(max(n, 0), 130)
+        for t in got.values():
+            assert not t[b, n:].any()
+
+
+def test_padding_may_hold_anything():
+    """Not a number and infinities in the padding of every input change nothing, in no output."""
+    lengths = [100, 3, 0, 65]
+    q, k, v, do = _qkv(4, 100, 100, 4, 2, 64, BF16, seed=5)
+    clean = _run(q, k, v, do, 30, 5, 2, lengths)
+    for t, bad in ((q, float("nan")), (k, float("inf")), (v, float("nan")), (do, float("-inf"))):
+        for b, n in enumerate(lengths):
+            t[b, n:] = bad
+    dirty = _run(q, k, v, do, 30, 5, 2, lengths)
+    for n in clean:
+        assert torch.equal(clean[n], dirty[n]), n
+
+
+@pytest.mark.parametrize("N,M,starts", [(1, 500, [499, 17]), (5, 300, [0, 295]), (64, 640, [576, 100]), (130, 1000, [870, 3]), (40, 30, [0, 0]), (10, 90, [85, 200])])
+def test_parts_of_a_prompt(N, M, starts):
+    """Queries behind cached keys; rows past the keys are padding."""
+    _check(*_qkv(2, N, M, 4, 1, 32, BF16, seed=M), 90, 0, 4, lengths=[min(M, s + N) for s in starts], starts=starts)
+
+
+def test_no_keys_and_no_queries():
+    from patchaugnet_amd.attention import window_attention
+    got = _run(*_qkv(2, 5, 0, 2, 2, 32, F32), None, 0, 0)
+    assert not got["out"].any() and not got["dq"].any() and got["dk"].shape == (2, 0, 2, 32)
+    got = _run(*_qkv(2, 0, 5, 2, 2, 32, F32), None, 0, 0)
+    assert got["out"].shape == (2, 0, 2, 32) and not got["dk"].any() and not got["dv"].any()
+    assert window_attention(*_qkv(0, 4, 4, 2, 2, 32, F32)[:3]).shape == (0, 4, 2, 32)
+
+
+def test_one_visible_key_returns_its_value():
+    q, k, v, do = _qkv(1, 200, 200, 2, 2, 64, F16)
+    got = _run(q, k, v, do, 0, 0, 0)
+    assert torch.equal(got["out"], v) and torch.equal(got["dv"], do)
+
+
+@pytest.mark.parametrize("amp", [40.0, 300.0])
+def test_large_scores(amp):
+    """Scores of thousands: one key takes all, the others underflow; nothing overflows."""
+    q, k, v, do = _qkv(1, 100, 100, 2, 2, 32, F32, seed=3)
+    got = _run(q * amp, k, v, do, 20, 20, 1)
+    val, tol = reference(q * amp, k, v, 20, 20, 1, dout=do)
+    for n in val:
+        close(got[n], val[n], tol[n], n)
+
+
+def test_growing_scores_rescale():
+    """Keys whose scores grow along the sequence move the running maximum in every tile, far beyond the range of one exponent."""
+    q, k, v, do = _qkv(1, 400, 400, 1, 1, 32, BF16, seed=4)
+    q, k = q.abs(), k.abs() * torch.linspace(0, 30, 400, device="cuda", dtype=BF16).view(1, -1, 1, 1)
+    _check(q, k, v, do, None, 0, 0)
+
+
+def test_views_of_one_projection():
+    """q, k, v as views of one (B, N, 3, H, D) tensor, a transposed batch, an expanded gradient; an unaligned view."""
+    from patchaugnet_amd.attention import window_attention
+    g = torch.Generator(device="cuda").manual_seed(9)
+    qkv = torch.randn(2, 90, 3, 4, 32, generator=g, device="cuda").to(BF16)
+    q, k, v = qkv.unbind(2)
+    do = torch.randn(4, 32, generator=g, device="cuda").to(BF16).expand(2, 90, 4, 32)
+    got = _check(q, k, v, do, 16, 0, 1)
+    assert torch.equal(got["out"], window_attention(q.contiguous(), k.contiguous(), v.contiguous(), left=16, sinks=1))
+    hn = q.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)                       # heads outside, tokens inside
+    assert torch.equal(got["out"], window_attention(hn, k, v, left=16, sinks=1))
+    wide = torch.zeros(2, 90, 4, 33, device="cuda", dtype=BF16)
+    wide[..., 1:] = q
+    assert torch.equal(got["out"], window_attention(wide[..., 1:], k, v, left=16, sinks=1))
+
+
+def test_same_bits_every_run_and_with_or_without_gradient():
+    from patchaugnet_amd.attention import window_attention
+    q, k, v, do = _qkv(2, 700, 700, 8, 1, 64, BF16, seed=1)
+    a = _run(q, k, v, do, 50, 0, 200)
+    for _ in range(3):
+        b = _run(q, k, v, do, 50, 0, 200)
+        for n in a:
+            assert torch.equal(a[n], b[n]), n
+    with torch.no_grad():
+        assert torch.equal(a["out"], window_attention(q, k, v, left=50, sinks=200))
+
+
+def test_few_rows_over_many_keys():
+    """Few queries over a long sequence: the keys are split over workgroups and joined; gradients of few keys seen by many rows."""
+    _check(*_qkv(1, 3, 5000, 4, 4, 64, F16, seed=8), None, 0, 0, lengths=[5000], starts=[4997])
+    _check(*_qkv(1, 3000, 3000, 1, 1, 32, F32, seed=8), 40, 0, 5)
+
+
+def test_gradients_against_differences():
+    """Directional differences of the 64-bit forward, step 2^-10: the third derivative's part is below 1e-6 of the sum of |gradient| |direction|."""
+    q, k, v, do = _qkv(1, 40, 40, 2, 1, 16, F32, seed=2)
+    got = _run(q, k, v, do, 12, 3, 2)
+    gen = torch.Generator(device="cuda").manual_seed(77)
+    for i, n in enumerate(("dq", "dk", "dv")):
+        d = torch.randn((q, k, v)[i].shape, generator=gen, device="cuda").double()
+        h = 2.0 ** -10
+        f = []
+        for sgn in (1, -1):
+            x = [t.double() for t in (q, k, v)]
+            x[i] = x[i] + sgn * h * d
+            out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+            from _attention_ref import seen
+            ok = seen(40, 40, 12, 3, 2, 40, 0, "cuda")
+            for hd in range(2):
+                s = (x[0][0, :, hd] @ x[1][0, :, 0].t().contiguous()) / 4.0
+                out[0, :, hd] = torch.softmax(s.masked_fill(~ok, float("-inf")), 1) @ x[2][0, :, 0]
+            f.append((out * do.double()).sum())
+        diff = (f[0] - f[1]) / (2 * h)
+        along = (got[n].double() * d).sum()
+        assert abs(float(diff - along)) <= 1e-5 * float((got[n].double() * d).abs().sum()), n
+
+
+def test_on_another_stream():
+    q, k, v, do = _qkv(2, 300, 300, 4, 2, 64, F16, seed=6)
+    want = _run(q, k, v, do, 33, 0, 2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _run(q, k, v, do, 33, 0, 2)
+    side.synchronize()
+    for n in want:
+        assert torch.equal(want[n], got[n]), n
+
+
+def test_captured_step_replays():
+    """A forward and backward pass captured into a graph, replayed between eager calls with new inputs, equals the eager results."""
+    q, k, v, do = _qkv(1, 600, 600, 8, 2, 64, BF16, seed=11)
+    lengths = _ints([600])
+    from patchaugnet_amd.attention import window_attention
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+
+    def step():
+        out = window_attention(*leaves, left=70, sinks=4, lengths=lengths)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, do)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for turn in range(4):
+        fresh = _qkv(1, 600, 600, 8, 2, 64, BF16, seed=20 + turn)
+        with torch.no_grad():
+            for t, f in zip(leaves, fresh):
+                t.copy_(f)
+        lengths.fill_(600 - 150 * turn)
+        graph.replay()
+        torch.cuda.synchronize()
+        held_now = [t.clone() for t in held]
+        want = _run(*fresh[:3], do, 70, 0, 4, lengths=[600 - 150 * turn])
+        for a, b in zip(held_now, want.values()):
+            assert torch.equal(a, b), turn
+
+
+def test_refusals():
+    from patchaugnet_amd.attention import window_attention
+    q, k, v, _ = _qkv(2, 20, 20, 4, 2, 32, F32)
+    for bad, exc in [
+            (lambda: window_attention(q.cpu(), k, v), RuntimeError), (lambda: window_attention(q, k.half(), v), TypeError),
+            (lambda: window_attention(q.double(), k.double(), v.double()), TypeError), (lambda: window_attention(q[0], k, v), ValueError),
+            (lambda: window_attention(q[:, :, :3], k, v), ValueError), (lambda: window_attention(q[..., :12], k[..., :12], v[..., :12]), ValueError),
+            (lambda: window_attention(q, k, v[:, :10]), ValueError), (lambda: window_attention(q, k[:1], v[:1]), ValueError),
+            (lambda: window_attention(q, k, v, left=-1), ValueError), (lambda: window_attention(q, k, v, right=1.5), ValueError),
+            (lambda: window_attention(q, k, v, sinks=-2), ValueError), (lambda: window_attention(q, k, v, scale=0.0), ValueError),
+            (lambda: window_attention(q, k, v, scale=float("nan")), ValueError), (lambda: window_attention(q, k, v, lengths=torch.tensor([1, 2])), ValueError),
+            (lambda: window_attention(q, k, v, lengths=_ints([1])), ValueError), (lambda: window_attention(q, k, v, q_start=_ints([[1], [2]])), ValueError)]:
+        with pytest.raises(exc):
+            bad()
+    leaf = q.clone().requires_grad_()
+    out = window_attention(leaf, k, v)
+    (g,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), leaf)
