@@ -30,7 +30,7 @@ struct FwdArgs {
 };
 
 template <typename T, int DT, bool SPLIT>
-__global__ __launch_bounds__(256) void fwd_kernel(const FwdArgs a)
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(const FwdArgs a)
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;

@@ -36,7 +36,7 @@ struct BwdArgs {
 };
 
 template <typename T, int DT>
-__global__ __launch_bounds__(256) void dq_kernel(const BwdArgs a)
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const BwdArgs a)
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
@@ -168,7 +168,7 @@ struct KeyTile {
 };
 
 template <typename T, int DT>
-__global__ __launch_bounds__(256) void dkv_kernel(const BwdArgs a)
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_kernel(const BwdArgs a)
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
