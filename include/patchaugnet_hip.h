@@ -529,7 +529,7 @@ int pa_qk_norm_rotary_backward(int dtype, int b, int n, int h, int hk, int d, co
                                float *dqw, float *dkw, float *scratch, pa_stream_t stream);
 
 /* out (b,n,h,d, contiguous) = softmax(scale q k^T over the keys in view) v; q (b,n,h,d), k and v (b,m,hk,d), d a multiple of 8 up to 128.
- * lse (b,h,n; NULL: not wanted): log2 of the sum of exponentials, for the backward pass.  scratch: as many floats as the function says (0: NULL). */
+ * kn, vn (backward: qn, qh, gn, gh too) <= 2^22.  lse (b,h,n; NULL: not wanted): log2 of the sum of exponentials, for the backward pass.  scratch: as many floats as the function says (0: NULL). */
 long pa_window_attention_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks);
 int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn, long kh,
                         const void *v, long vb, long vn, long vh, int left, int right, int sinks, float scale, const int *start, const int *length, void *out,

@@ -26,6 +26,7 @@ from ._lib import call, ptr
 __all__ = ["qk_norm_rotary", "window_attention", "paged_append", "paged_attention"]
 
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_FAR = 1 << 22             # elements between neighbouring tokens or heads: 32-bit offsets inside a tile (pa_attn.h)
 _PTYPE = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _MAXLEN = 1 << 28            # tokens of a sequence (pa_attn.h)
 
@@ -54,10 +55,12 @@ def _ints(name, what, t, device, n):
     return t.contiguous()
 
 
-def _rows(t, align=16):
-    """t itself if its last dimension is contiguous and every row starts at a multiple of `align` bytes, else a contiguous copy."""
+def _rows(t, align=16, far=1 << 62):
+    """t itself if its last dimension is contiguous, every row starts at a multiple of `align` bytes and those of neighbouring tokens and heads lie at most
+    `far` elements apart, else a contiguous copy."""
     es = t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % align == 0 and all(s * es % align == 0 and s >= 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+    if t.stride(-1) == 1 and t.data_ptr() % align == 0 and all(s * es % align == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1) \
+            and all(s <= far for s, n in zip(t.stride()[1:-1], t.shape[1:-1]) if n > 1) and (far > _FAR or t.shape[-2] * t.stride(-2) * 4 < 1 << 31):
         return t
     return t.contiguous()
 
@@ -210,7 +213,7 @@ class _WindowAttention(Function):
     @once_differentiable
     def backward(ctx, g):
         q, k, v, start, length, out, lse = ctx.saved_tensors
-        g = _rows(g)
+        g = _rows(g, far=_FAR)
         left, right, sinks, scale = ctx.view
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         B, N, H, D = q.shape
@@ -231,7 +234,7 @@ def window_attention(q, k, v, *, left=None, right=0, sinks=0, scale=None, length
                 q, k, v holds has no influence, NaN included.  Within a sequence a NaN or an infinity reaches rows that do not see it.
       q_start   int32 (B,): position of the first query (None: 0) -- the next part of a prompt, whose earlier keys lie in front of it in k and v.
     Values outside 0..M are clamped.  scale None: 1 / sqrt(D).  Strides are free except that a row is contiguous and starts at a multiple of 16 bytes
-    (other tensors are copied).  Gradients for q, k, v, the same bits on every run."""
+    (other tensors are copied; so are those with 2^22 elements and more between two tokens).  Gradients for q, k, v, the same bits on every run."""
     name = "window_attention"
     _check(name, q, k, v)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
@@ -240,7 +243,7 @@ def window_attention(q, k, v, *, left=None, right=0, sinks=0, scale=None, length
     left, right, sinks = _side(name, "left", left), _side(name, "right", right), max(_side(name, "sinks", sinks), 0)
     view = (left, right, sinks, _scale(name, scale, q.shape[3]))
     length, start = _ints(name, "lengths", lengths, q.device, q.shape[0]), _ints(name, "q_start", q_start, q.device, q.shape[0])
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    q, k, v = (_rows(t, far=_FAR) for t in (q, k, v))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowAttention.apply(q, k, v, start, length, view)
     return _window_forward(q, k, v, start, length, view, False)[0]

@@ -29,6 +29,14 @@ constexpr int MAXLEN = 1 << 28;          // tokens of a sequence, rows of a key 
 constexpr int UNBOUNDED = 1 << 29;       // window side without a limit
 constexpr int NOWHERE = 0x7fffffff;      // a position that no key reaches
 
+// Workgroups go to the eight XCDs in turn; each XCD has an L2 of its own.  Work item for workgroup x of n, such that an XCD's workgroups own one
+// contiguous run of items: neighbours, which share keys and values, meet in one L2.
+__device__ __forceinline__ long xcd_item(long x, long n)
+{
+    const long k = x & 7, each = n >> 3, rest = n & 7;
+    return k * each + (k < rest ? k : rest) + (x >> 3);
+}
+
 template <typename T> struct Frag;
 template <> struct Frag<float> { typedef pa_f8 type; };
 template <> struct Frag<_Float16> { typedef pa_h8 type; };
@@ -109,6 +117,55 @@ template <typename T, int DT> struct Tile {
     }
 };
 
+// 16 bytes of a row from global memory, zeros when `ok` is false (the address is not touched then)
+__device__ __forceinline__ pa_u4 ldg16(const void *p, bool ok)
+{
+    pa_u4 z = {0, 0, 0, 0};
+    if (ok) z = *reinterpret_cast<const pa_u4 *>(p);
+    return z;
+}
+
+// R rows of a tensor on their way into an LDS tile: 256 threads, 16-byte chunks, fetched into registers and stored later.  A thread's places in a tile
+// are the same for every tile, so a fetch is one load per chunk at (uniform base of the tile) + (32-bit offset of the thread); rows from `valid` on and
+// elements from d on arrive as zeros, whatever is in memory there (checked only for tiles and widths that have any).
+template <typename T, int DT, int R> struct Stage {
+    typedef Tile<T, DT> L;
+    static constexpr int N = R * L::CH / 256;
+    static_assert(R * L::CH % 256 == 0, "a tile splits evenly over the workgroup");
+    u32 off[N];
+    pa_u4 x[N];
+
+    __device__ static __forceinline__ int row(int u) { return (int)(threadIdx.x + u * 256) / L::CH; }
+    __device__ static __forceinline__ int chunk(int u) { return (int)(threadIdx.x + u * 256) - row(u) * L::CH; }
+    // rows `stride` elements apart
+    __device__ __forceinline__ void strided(long stride)
+    {
+#pragma unroll
+        for (int u = 0; u < N; ++u) off[u] = ((u32)row(u) * (u32)stride + chunk(u) * L::EC) * (u32)sizeof(T);
+    }
+    __device__ __forceinline__ void fetch(const T *base, int valid, int d)
+    {
+        const char *p = reinterpret_cast<const char *>(base);
+        if (valid >= R && d == DT) {
+#pragma unroll
+            for (int u = 0; u < N; ++u) x[u] = *reinterpret_cast<const pa_u4 *>(p + off[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u) {                       // row 0, chunk 0 is always there (valid >= 1): no branch around the load
+                const bool ok = row(u) < valid && chunk(u) * L::EC < d;
+                const pa_u4 t = *reinterpret_cast<const pa_u4 *>(p + (ok ? off[u] : 0u));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[u][i] = ok ? t[i] : 0u;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char *s) const
+    {
+#pragma unroll
+        for (int u = 0; u < N; ++u) *reinterpret_cast<pa_u4 *>(s + L::at(row(u), chunk(u))) = x[u];
+    }
+};
+
 // eight accumulator registers as an operand fragment (one rounding to the operand type)
 template <typename T> __device__ __forceinline__ typename Frag<T>::type pack(const pa_f16v &a, int u)
 {
@@ -116,14 +173,6 @@ template <typename T> __device__ __forceinline__ typename Frag<T>::type pack(con
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = (T)a[8 * u + e];
     return f;
-}
-
-// 16 bytes of a row from global memory, zeros when `ok` is false (the address is not touched then)
-__device__ __forceinline__ pa_u4 ldg16(const void *p, bool ok)
-{
-    pa_u4 z = {0, 0, 0, 0};
-    if (ok) z = *reinterpret_cast<const pa_u4 *>(p);
-    return z;
 }
 
 // fragment of a row held in global memory: elements 16 kk + 8 h .. of `row`, zeros past d (a multiple of 8)
@@ -222,6 +271,9 @@ static inline int window_attention_check(const char *name, int dtype, int b, int
     PA_REQUIRE(scale > 0.f && scale < INFINITY, "%s: the scale has to be positive and finite", name);
     return PA_OK;
 }
+
+// a tile's rows are addressed by 32-bit offsets: 64 tokens and 64 heads of 4-byte elements stay below 2^32 bytes
+constexpr long PA_ATTN_MAXSTRIDE = 1l << 22;
 
 // element type and padded head width as template arguments of F: runs F(T, DT)
 #define PA_ATTN_WIDTH(T, d, F)                                                  \

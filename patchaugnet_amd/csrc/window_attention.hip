@@ -34,12 +34,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(const 
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
-    constexpr int NF = KT * L::CH / 256;                       // chunks a thread stages per tensor
     constexpr int TB = KT * L::RB;
     extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K tile, V tile]
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
 
-    const int qt = blockIdx.x % a.nqt, bh = blockIdx.x / a.nqt, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int item = (int)xcd_item(blockIdx.x, gridDim.x);
+    const int qt = item % a.nqt, bh = item / a.nqt, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int rows = a.N * a.G, len = a.view.len(b), start = a.view.first(b);
     const int r0 = qt * QT;
     const TileList<KT> tiles(a.view, start + a.g.div(r0), start + a.g.div(min(r0 + QT, rows) - 1), len);
@@ -66,15 +66,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(const 
     const int flo = max(wp1 - a.view.left, 0), fhi = min(wp0 + a.view.right, len - 1);                  // every row sees [flo, fhi]
 
     const T *kp = (const T *)a.k + b * a.kb + hk * a.kh, *vp = (const T *)a.v + b * a.vb + hk * a.vh;
-    pa_u4 pk[NF], pv[NF];
-    auto fetch = [&](int t) {
-#pragma unroll
-        for (int u = 0; u < NF; ++u) {
-            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH, j = t * KT + r;
-            const bool ok = j < len && c * L::EC < a.D;        // rows behind the sequence are zeros: what they hold never meets a product
-            pk[u] = ldg16(kp + (long)j * a.kn + c * L::EC, ok);
-            pv[u] = ldg16(vp + (long)j * a.vn + c * L::EC, ok);
-        }
+    Stage<T, DT, KT> sk, sv;
+    sk.strided(a.kn);
+    sv.strided(a.vn);
+    auto fetch = [&](int t) {                                  // rows behind the sequence are zeros: what they hold never meets a product
+        sk.fetch(kp + (long)t * KT * a.kn, len - t * KT, a.D);
+        sv.fetch(vp + (long)t * KT * a.vn, len - t * KT, a.D);
     };
 
     pa_f16v o[DT / 32];
@@ -85,12 +82,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(const 
     if (t0 < t1) fetch(tiles.tile(t0));
     for (int it = t0; it < t1; ++it) {
         char *ks = smem + ((it - t0) & 1) * 2 * TB, *vs = ks + TB;
-#pragma unroll
-        for (int u = 0; u < NF; ++u) {
-            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH;
-            *reinterpret_cast<pa_u4 *>(ks + L::at(r, c)) = pk[u];
-            *reinterpret_cast<pa_u4 *>(vs + L::at(r, c)) = pv[u];
-        }
+        sk.store(ks);
+        sv.store(vs);
         __syncthreads();                                       // the previous tile's readers of this half passed the barrier before this one
         const int j0 = tiles.tile(it) * KT;
         if (it + 1 < t1) fetch(tiles.tile(it + 1));
@@ -247,6 +240,7 @@ PA_API int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, in
     a.g = Div(a.G);
     a.nqt = pa_div_up((long)n * a.G, QT);
     a.splits = fwd_splits(b, n, m, h, hk, a.view.left, a.view.right, sinks);
+    PA_REQUIRE(kn >= 0 && vn >= 0 && kn <= PA_ATTN_MAXSTRIDE && vn <= PA_ATTN_MAXSTRIDE, "pa_window_attention: tokens are more than 2^22 elements apart");
     PA_REQUIRE((long)a.nqt * b * hk < (1l << 31), "pa_window_attention: too many workgroups");
     PA_REQUIRE(a.splits == 1 || scratch, "pa_window_attention: this size needs pa_window_attention_scratch_floats() of scratch");
     hipStream_t st = (hipStream_t)stream;

@@ -30,6 +30,7 @@ struct BwdArgs {
     long qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh;
     int B, N, H, Hk, D, G, nqt;
     int nst, nkt, ssink, snorm;        // key tiles with first tokens, all key tiles, slices of either kind
+    int rt;                            // rows of a tile: as many whole queries as fit
     float c, scale;
     View view;
     Div g;
@@ -40,10 +41,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const B
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
-    constexpr int NF = KT * L::CH / 256, TB = KT * L::RB;
+    constexpr int TB = KT * L::RB;
     extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K tile, V tile]
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
-    const int qt = blockIdx.x % a.nqt, bh = blockIdx.x / a.nqt, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int item = (int)xcd_item(blockIdx.x, gridDim.x);
+    const int qt = item % a.nqt, bh = item / a.nqt, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int rows = a.N * a.G, len = a.view.len(b), start = a.view.first(b);
     const int r0 = qt * QT;
 
@@ -75,15 +77,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const B
     const int flo = max(wp1 - a.view.left, 0), fhi = min(wp0 + a.view.right, len - 1);
 
     const T *kp = (const T *)a.k + b * a.kb + hk * a.kh, *vp = (const T *)a.v + b * a.vb + hk * a.vh;
-    pa_u4 pk[NF], pv[NF];
+    Stage<T, DT, KT> sk, sv;
+    sk.strided(a.kn);
+    sv.strided(a.vn);
     auto fetch = [&](int t) {
-#pragma unroll
-        for (int u = 0; u < NF; ++u) {
-            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH, j = t * KT + r;
-            const bool ok = j < len && c * L::EC < a.D;
-            pk[u] = ldg16(kp + (long)j * a.kn + c * L::EC, ok);
-            pv[u] = ldg16(vp + (long)j * a.vn + c * L::EC, ok);
-        }
+        sk.fetch(kp + (long)t * KT * a.kn, len - t * KT, a.D);
+        sv.fetch(vp + (long)t * KT * a.vn, len - t * KT, a.D);
     };
 
     pa_f16v dq[DT / 32];
@@ -94,12 +93,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const B
     if (tiles.n) fetch(tiles.tile(0));
     for (int it = 0; it < tiles.n; ++it) {
         char *ks = smem + (it & 1) * 2 * TB, *vs = ks + TB;
-#pragma unroll
-        for (int u = 0; u < NF; ++u) {
-            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH;
-            *reinterpret_cast<pa_u4 *>(ks + L::at(r, c)) = pk[u];
-            *reinterpret_cast<pa_u4 *>(vs + L::at(r, c)) = pv[u];
-        }
+        sk.store(ks);
+        sv.store(vs);
         __syncthreads();
         const int j0 = tiles.tile(it) * KT;
         if (it + 1 < tiles.n) fetch(tiles.tile(it + 1));
@@ -172,10 +167,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_k
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
-    constexpr int NF = RT * L::CH / 256, TB = RT * L::RB, BUF = 2 * TB + 3 * RT * 4;
+    constexpr int TB = RT * L::RB, BUF = 2 * TB + 3 * RT * 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][Q tile, dO tile, lse, delta, position]
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
-    const KeyTile kt(a, blockIdx.x);
+    const KeyTile kt(a, xcd_item(blockIdx.x, gridDim.x));
     const int b = kt.bh / a.Hk, hk = kt.bh - b * a.Hk;
     const int len = a.view.len(b), start = a.view.first(b);
     const int k0 = kt.tile * KB, k1 = min(k0 + KB, len) - 1;
@@ -190,7 +185,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_k
             rb = (ib + 1) * a.G;
         }
     }
-    const int all = (rb - ra + RT - 1) / RT;
+    const int all = (rb - ra + a.rt - 1) / a.rt;
     const int t0 = (int)((long)all * kt.slice / kt.slices), t1 = (int)((long)all * (kt.slice + 1) / kt.slices);
 
     const int wk = __builtin_amdgcn_readfirstlane(k0 + wave * 32), wk1 = min(wk + 31, len - 1);
@@ -209,23 +204,37 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_k
         }
     }
 
-    pa_u4 pq[NF], pg[NF];
+    // A tile is a.rt rows: whole queries, so that a thread's rows have the same head and the same distance from the tile's first query every time.
+    // (More than RT heads a group: RT rows from anywhere, decoded each time.)
+    Stage<T, DT, RT> sq, sg;
+    const bool whole = a.G <= RT;
     float pl = 0.f, pd = 0.f;
     int pp = 0;
-    auto fetch = [&](int t) {
+    const T *qp = (const T *)a.q + b * a.qb + hk * a.G * a.qh, *gp = (const T *)a.dout + b * a.gb + hk * a.G * a.gh;
+    auto place = [&](int first) {                              // offsets of the tile's rows from query first / G
 #pragma unroll
-        for (int u = 0; u < NF; ++u) {
-            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH, row = ra + t * RT + r;
-            const int i = a.g.div(min(row, rb - 1)), hq = hk * a.G + row - i * a.G;
-            const bool ok = row < rb && c * L::EC < a.D;       // padding rows are behind rb
-            pq[u] = ldg16((const T *)a.q + b * a.qb + i * a.qn + hq * a.qh + c * L::EC, ok);
-            pg[u] = ldg16((const T *)a.dout + b * a.gb + i * a.gn + hq * a.gh + c * L::EC, ok);
+        for (int u = 0; u < sq.N; ++u) {
+            const int x = first + sq.row(u), i = a.g.div(x), g = x - i * a.G;
+            sq.off[u] = ((u32)i * (u32)a.qn + (u32)g * (u32)a.qh + sq.chunk(u) * L::EC) * (u32)sizeof(T);
+            sg.off[u] = ((u32)i * (u32)a.gn + (u32)g * (u32)a.gh + sq.chunk(u) * L::EC) * (u32)sizeof(T);
         }
+    };
+    place(0);
+    const int li = a.g.div(tid), lg = hk * a.G + tid - li * a.G;       // row tid of a tile: query and head (threads below RT)
+    auto fetch = [&](int t) {
+        const int first = ra + t * a.rt, i0 = a.g.div(first), valid = min(a.rt, rb - first);
+        if (!whole) place(first - i0 * a.G);
+        sq.fetch(qp + (long)i0 * a.qn, valid, a.D);            // padding rows are behind rb
+        sg.fetch(gp + (long)i0 * a.gn, valid, a.D);
         if (tid < RT) {
-            const int row = ra + t * RT + tid, i = a.g.div(min(row, rb - 1)), hq = hk * a.G + row - i * a.G;
+            int i = i0 + li, hq = lg;
+            if (!whole) {
+                i = a.g.div(first + tid);
+                hq = hk * a.G + first + tid - i * a.G;
+            }
             const size_t at = ((size_t)b * a.H + hq) * a.N + i;
-            pl = row < rb ? a.lse[at] : INFINITY;
-            pd = row < rb ? a.delta[at] : 0.f;
+            pl = tid < valid ? a.lse[at] : INFINITY;
+            pd = tid < valid ? a.delta[at] : 0.f;
             pp = start + i;
         }
     };
@@ -239,12 +248,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_k
         char *qs = smem + ((t - t0) & 1) * BUF, *gs = qs + TB;
         float *ls = reinterpret_cast<float *>(gs + TB), *ds = ls + RT;
         int *ps = reinterpret_cast<int *>(ds + RT);
-#pragma unroll
-        for (int u = 0; u < NF; ++u) {
-            const int idx = tid + u * 256, r = idx / L::CH, c = idx - r * L::CH;
-            *reinterpret_cast<pa_u4 *>(qs + L::at(r, c)) = pq[u];
-            *reinterpret_cast<pa_u4 *>(gs + L::at(r, c)) = pg[u];
-        }
+        sq.store(qs);
+        sg.store(gs);
         if (tid < RT) {
             ls[tid] = pl;
             ds[tid] = pd;
@@ -255,9 +260,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_k
         if (!wave_on) continue;
 #pragma unroll
         for (int sub = 0; sub < RT / 32; ++sub) {
-            const int rs = ra + t * RT + sub * 32;
-            if (rs >= rb) continue;
-            const int p0 = start + a.g.div(rs), p1 = start + a.g.div(min(rs + 31, rb - 1));
+            const int rs = ra + t * a.rt + sub * 32, re = min(min(rs + 31, ra + t * a.rt + a.rt - 1), rb - 1);
+            if (rs > re) continue;
+            const int p0 = start + a.g.div(rs), p1 = start + a.g.div(re);
             if (!(p1 >= wk - a.view.right && (p0 <= wk1 + a.view.left || wk < a.view.sinks))) continue;
             pa_f16v s = (pa_f16v)(0.f), dp = (pa_f16v)(0.f);
 #pragma unroll
@@ -355,7 +360,7 @@ Slices slices_of(int B, int N, int M, int H, int Hk, int left, int right, int si
     s.nkt = pa_div_up(M, KB);
     const long sk = sinks < M ? sinks : M;
     s.nst = pa_div_up(sk, KB);
-    const long wgs = (long)B * Hk * s.nkt, reach = (long)left + right + KB, walk = pa_div_up((N < reach ? N : reach) * G, RT), whole = pa_div_up(N * G, RT);
+    const long wgs = (long)B * Hk * s.nkt, reach = (long)left + right + KB, rt = G <= RT ? RT / G * G : RT, walk = pa_div_up((N < reach ? N : reach) * G, rt), whole = pa_div_up(N * G, rt);
     long n = wgs ? 512 / wgs : 1;
     if (n > walk / 4) n = walk / 4;
     s.snorm = n < 1 ? 1 : n > 64 ? 64 : (int)n;
@@ -417,7 +422,12 @@ PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, i
     a.g = Div(a.G);
     a.nqt = pa_div_up((long)n * a.G, QT);
     const Slices s = slices_of(b, n, m, h, hk, a.view.left, a.view.right, sinks);
+    a.rt = a.G <= RT ? RT / a.G * a.G : RT;
     a.nst = s.nst; a.nkt = s.nkt; a.ssink = s.ssink; a.snorm = s.snorm;
+    PA_REQUIRE(kn >= 0 && vn >= 0 && kn <= PA_ATTN_MAXSTRIDE && vn <= PA_ATTN_MAXSTRIDE && qn >= 0 && qh >= 0 && gn >= 0 && gh >= 0 && qn <= PA_ATTN_MAXSTRIDE &&
+                   gn <= PA_ATTN_MAXSTRIDE && qh <= PA_ATTN_MAXSTRIDE && gh <= PA_ATTN_MAXSTRIDE,
+               "pa_window_attention_backward: tokens or heads are more than 2^22 elements apart");
+    PA_REQUIRE(a.G <= RT || (long)a.G * (qh > gh ? qh : gh) * 4 < (1l << 31), "pa_window_attention_backward: the heads of a group span 2^31 bytes");
     PA_REQUIRE((long)a.nqt * b * hk < (1l << 31) && (long)b * hk * ((long)s.nst * s.ssink + (long)(s.nkt - s.nst) * s.snorm) * 32 < (1l << 31),
                "pa_window_attention_backward: too many workgroups");
     hipStream_t st = (hipStream_t)stream;
