@@ -125,18 +125,18 @@ __device__ __forceinline__ pa_u4 ldg16(const void *p, bool ok)
     return z;
 }
 
-// R rows of a tensor on their way into an LDS tile: 256 threads, 16-byte chunks, fetched into registers and stored later.  A thread's places in a tile
+// R rows of a tensor on their way into an LDS tile: NT threads, 16-byte chunks, fetched into registers and stored later.  A thread's places in a tile
 // are the same for every tile, so a fetch is one load per chunk at (uniform base of the tile) + (32-bit offset of the thread); rows from `valid` on and
 // elements from d on arrive as zeros, whatever is in memory there (checked only for tiles and widths that have any).
-template <typename T, int DT, int R> struct Stage {
+template <typename T, int DT, int R, int NT> struct Stage {
     typedef Tile<T, DT> L;
-    static constexpr int N = R * L::CH / 256;
-    static_assert(R * L::CH % 256 == 0, "a tile splits evenly over the workgroup");
+    static constexpr int N = R * L::CH / NT;
+    static_assert(R * L::CH % NT == 0, "a tile splits evenly over the workgroup");
     u32 off[N];
     pa_u4 x[N];
 
-    __device__ static __forceinline__ int row(int u) { return (int)(threadIdx.x + u * 256) / L::CH; }
-    __device__ static __forceinline__ int chunk(int u) { return (int)(threadIdx.x + u * 256) - row(u) * L::CH; }
+    __device__ static __forceinline__ int row(int u) { return (int)(threadIdx.x + u * NT) / L::CH; }
+    __device__ static __forceinline__ int chunk(int u) { return (int)(threadIdx.x + u * NT) - row(u) * L::CH; }
     // rows `stride` elements apart
     __device__ __forceinline__ void strided(long stride)
     {
@@ -253,6 +253,13 @@ template <int KT> struct TileList {
     }
     __device__ __forceinline__ int tile(int i) const { return i < nsk ? i : lo + i - nsk; }
 };
+
+// Waves of a workgroup, each with 32 rows (or keys): four share a tile's way into LDS; two make the grid finer, which counts while there are few
+// rounds of workgroups, since the last round is seldom full.  `four`: workgroups of four waves that the problem makes.
+static inline int waves_of(long four) { return four < 2048 ? 2 : 4; }
+
+// Keys of a tile of the kernels that own rows: fewer where two waves alone bring wide rows into LDS (registers).
+template <typename T, int DT, int NW> constexpr int key_tile() { return NW == 2 && DT * (int)sizeof(T) >= 256 ? 32 : 64; }
 
 static inline int width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }      // padded head width
 

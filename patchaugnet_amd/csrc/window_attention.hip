@@ -2,7 +2,7 @@
 //
 //     o_i = sum_j P_ij v_j,   P_ij = exp(s_ij) / sum_j exp(s_ij),   s_ij = scale q_i . k_j   over the keys j in view of row i (View, pa_attn.h)
 //
-// One pass over the keys with a running maximum and sum: O(window) work and nothing N x M in memory.  A workgroup owns 128 rows -- the N queries of
+// One pass over the keys with a running maximum and sum: O(window) work and nothing N x M in memory.  A workgroup owns 128 (64) rows -- the N queries of
 // the G heads that share a key head, query-major, so that one tile of keys serves all of them -- and walks the 64-key tiles that its rows can see:
 // the tiles of the first tokens, then one contiguous range.  A wave owns 32 rows.  S^T = K Q^T puts one row into a lane's registers (maximum and
 // sum need one exchange between the two half waves), and the registers of P^T feed O^T += V^T P^T without leaving the lane; V is read transposed
@@ -16,8 +16,6 @@ using namespace pa_attn;
 
 namespace {
 
-constexpr int QT = 128, KT = 64;
-
 struct FwdArgs {
     const void *q, *k, *v;
     void *out;
@@ -29,12 +27,12 @@ struct FwdArgs {
     Div g;
 };
 
-template <typename T, int DT, bool SPLIT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(const FwdArgs a)
+template <typename T, int DT, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(const FwdArgs a)
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
-    constexpr int TB = KT * L::RB;
+    constexpr int KT = key_tile<T, DT, NW>(), TB = KT * L::RB, QT = 32 * NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K tile, V tile]
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
 
@@ -66,7 +64,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(const 
     const int flo = max(wp1 - a.view.left, 0), fhi = min(wp0 + a.view.right, len - 1);                  // every row sees [flo, fhi]
 
     const T *kp = (const T *)a.k + b * a.kb + hk * a.kh, *vp = (const T *)a.v + b * a.vb + hk * a.vh;
-    Stage<T, DT, KT> sk, sv;
+    Stage<T, DT, KT, 64 * NW> sk, sv;
     sk.strided(a.kn);
     sv.strided(a.vn);
     auto fetch = [&](int t) {                                  // rows behind the sequence are zeros: what they hold never meets a product
@@ -182,32 +180,48 @@ __global__ __launch_bounds__(256) void join_kernel(const FwdArgs a)
     if (a.lse && c == 0) a.lse[((size_t)b * a.H + hq) * a.N + i] = inv == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
+struct Shape {
+    int waves, nqt, splits;
+};
+
 // Work is split over the keys when the rows alone leave the chip idle: fewer than 256 workgroups (one per CU).  Two per CU are aimed at, each with
 // at least four tiles, because a part costs one round trip of its rows in 32 bits.
-int fwd_splits(int B, int N, int M, int H, int Hk, int left, int right, int sinks)
+Shape shape_of(int B, int N, int M, int H, int Hk, int left, int right, int sinks)
 {
-    const long G = H / Hk, wgs = (long)B * Hk * pa_div_up((long)N * G, QT);
-    if (wgs >= 256) return 1;
-    const long span = (long)left + right + QT / G + 1;                       // longest range of keys of one workgroup
-    const long tiles = pa_div_up(M < span ? M : span, KT) + (left < M ? pa_div_up(sinks, KT) : 0);
+    const long G = H / Hk, rows = (long)N * G;
+    Shape s;
+    s.waves = waves_of((long)B * Hk * ((rows + 127) / 128));
+    s.nqt = pa_div_up(rows, 32 * s.waves);
+    s.splits = 1;
+    const long wgs = (long)B * Hk * s.nqt;
+    if (wgs >= 256) return s;
+    const long span = (long)left + right + 32 * s.waves / G + 1;             // longest range of keys of one workgroup
+    const long tiles = pa_div_up(M < span ? M : span, 64) + (left < M ? pa_div_up(sinks, 64) : 0);
     const long want = 512 / wgs, most = tiles / 4;
-    const long s = want < most ? want : most;
-    return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
+    const long n = want < most ? want : most;
+    s.splits = n < 1 ? 1 : (n > 64 ? 64 : (int)n);
+    return s;
+}
+
+template <typename T, int DT, int NW, bool SPLIT>
+void launch_rows(const FwdArgs &a, hipStream_t st)
+{
+    constexpr int lds = 4 * key_tile<T, DT, NW>() * DT * (int)sizeof(T);
+    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&fwd_kernel<T, DT, NW, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipLaunchKernelGGL((fwd_kernel<T, DT, NW, SPLIT>), dim3((unsigned)((long)a.nqt * a.B * a.Hk), (unsigned)a.splits), dim3(64 * NW), lds, st, a);
 }
 
 template <typename T, int DT>
-int launch_fwd(const FwdArgs &a, hipStream_t st)
+int launch_fwd(const FwdArgs &a, int waves, hipStream_t st)
 {
-    constexpr int lds = 4 * KT * DT * (int)sizeof(T);
-    const dim3 grid((unsigned)((long)a.nqt * a.B * a.Hk), (unsigned)a.splits);
-    if (a.splits > 1) {
-        if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&fwd_kernel<T, DT, true>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        hipLaunchKernelGGL((fwd_kernel<T, DT, true>), grid, dim3(256), lds, st, a);
+    if (a.splits > 1) {                                        // few rows: always two waves
+        launch_rows<T, DT, 2, true>(a, st);
         const long threads = (long)a.B * a.Hk * a.N * a.G * (DT / 4);
         hipLaunchKernelGGL((join_kernel<T, DT>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+    } else if (waves == 2) {
+        launch_rows<T, DT, 2, false>(a, st);
     } else {
-        if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&fwd_kernel<T, DT, false>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        hipLaunchKernelGGL((fwd_kernel<T, DT, false>), grid, dim3(256), lds, st, a);
+        launch_rows<T, DT, 4, false>(a, st);
     }
     return 0;
 }
@@ -218,7 +232,7 @@ PA_API long pa_window_attention_scratch_floats(int b, int n, int m, int h, int h
 {
     if (b <= 0 || n <= 0 || h <= 0 || hk <= 0 || h % hk != 0) return 0;
     const int l = left < 0 ? UNBOUNDED : left, r = right < 0 ? UNBOUNDED : right;
-    const int s = fwd_splits(b, n, m, h, hk, l, r, sinks);
+    const int s = shape_of(b, n, m, h, hk, l, r, sinks).splits;
     return s <= 1 ? 0 : (long)s * b * n * h * (width(d) + 2);
 }
 
@@ -238,13 +252,14 @@ PA_API int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, in
     a.view.start = start; a.view.length = length;
     a.c = scale * 1.4426950408889634f;
     a.g = Div(a.G);
-    a.nqt = pa_div_up((long)n * a.G, QT);
-    a.splits = fwd_splits(b, n, m, h, hk, a.view.left, a.view.right, sinks);
+    const Shape sh = shape_of(b, n, m, h, hk, a.view.left, a.view.right, sinks);
+    a.nqt = sh.nqt;
+    a.splits = sh.splits;
     PA_REQUIRE(kn >= 0 && vn >= 0 && kn <= PA_ATTN_MAXSTRIDE && vn <= PA_ATTN_MAXSTRIDE, "pa_window_attention: tokens are more than 2^22 elements apart");
     PA_REQUIRE((long)a.nqt * b * hk < (1l << 31), "pa_window_attention: too many workgroups");
     PA_REQUIRE(a.splits == 1 || scratch, "pa_window_attention: this size needs pa_window_attention_scratch_floats() of scratch");
     hipStream_t st = (hipStream_t)stream;
-#define FWD(T, DT) launch_fwd<T, DT>(a, st)
+#define FWD(T, DT) launch_fwd<T, DT>(a, sh.waves, st)
     PA_ATTN_DISPATCH(dtype, d, FWD);
 #undef FWD
     PA_CHECK_LAUNCH("pa_window_attention");

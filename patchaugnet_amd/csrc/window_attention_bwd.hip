@@ -8,8 +8,9 @@
 // owner in a fixed order: no atomics, the same bits every run.  The registers of P and dS feed the second products as they are (pa_attn.h); q, do
 // and k are read from LDS both as rows and transposed.
 //
-// The keys of the first tokens are seen by every later row, so their walk is N / window times longer than any other's: it is cut into slices that
-// write 32-bit partial sums, joined by a second launch; so are all walks when the keys alone do not fill the chip.
+// The first tokens are seen by every later row, N / window times more rows than see any other key.  The rows behind their window are walked by
+// workgroups of their own, 32 keys each: there the waves share the keys and take the rows in turn.  They write 32-bit partial sums, joined with the
+// window's by a second launch; all walks are cut into such slices when the keys alone do not fill the chip.
 //
 // Roundings: P and dS are rounded to the operand type for the second products (16-bit types); the scale is applied to the 32-bit sums, so that dS is
 // rounded before it gets smaller.
@@ -19,8 +20,8 @@ using namespace pa_attn;
 
 namespace {
 
-constexpr int QT = 128, KT = 64;       // dq: rows of a workgroup, keys of a tile
-constexpr int KB = 128, RT = 64;       // dk, dv: keys of a workgroup, rows of a tile
+// dk, dv: rows of a tile, fewer where they are wide (registers on their way into LDS)
+template <typename T, int DT> constexpr int row_tile() { return DT * (int)sizeof(T) >= 512 ? 32 : 64; }
 
 struct BwdArgs {
     const void *q, *k, *v, *out, *dout;
@@ -29,19 +30,20 @@ struct BwdArgs {
     void *dq, *dk, *dv;
     long qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh;
     int B, N, H, Hk, D, G, nqt;
-    int nst, nkt, ssink, snorm;        // key tiles with first tokens, all key tiles, slices of either kind
+    int nkt, slices;                   // key tiles, slices of their walks
+    int nst, groups, fars;             // key tiles with first tokens, groups of 32 first tokens that have far rows, slices of their walks
     int rt;                            // rows of a tile: as many whole queries as fit
     float c, scale;
     View view;
     Div g;
 };
 
-template <typename T, int DT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const BwdArgs a)
+template <typename T, int DT, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const BwdArgs a)
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
-    constexpr int TB = KT * L::RB;
+    constexpr int KT = key_tile<T, DT, NW>(), TB = KT * L::RB, QT = 32 * NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K tile, V tile]
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
     const int item = (int)xcd_item(blockIdx.x, gridDim.x);
@@ -77,7 +79,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const B
     const int flo = max(wp1 - a.view.left, 0), fhi = min(wp0 + a.view.right, len - 1);
 
     const T *kp = (const T *)a.k + b * a.kb + hk * a.kh, *vp = (const T *)a.v + b * a.vb + hk * a.vh;
-    Stage<T, DT, KT> sk, sv;
+    Stage<T, DT, KT, 64 * NW> sk, sv;
     sk.strided(a.kn);
     sv.strided(a.vn);
     auto fetch = [&](int t) {
@@ -135,60 +137,65 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const B
         }
 }
 
-// what a workgroup of the dk, dv launch owns: the slices of the first tokens' tiles come first (they are the longest walks)
-struct KeyTile {
-    int bh, tile, slice, slices;
-    long slot;                          // place of its partial sums; < 0: it writes the gradients itself
+// What a workgroup of the dk, dv launch owns: a slice of the far rows of 32 first tokens (these come first), or a slice of a key tile's window.
+struct Walk {
+    int bh, k0, slice, slices;          // keys from k0
+    bool far;
+    long slot;                          // place of its partial sums, in keys; < 0: it writes the gradients itself
 
-    __device__ __forceinline__ KeyTile(const BwdArgs &a, long id)
+    __device__ __forceinline__ Walk(const BwdArgs &a, long id, int kb, int nw)
     {
-        const long nsink = (long)a.B * a.Hk * a.nst * a.ssink;
-        if (id < nsink) {
-            slices = a.ssink;
-            slot = slices > 1 ? id : -1;
+        const long nfar = (long)a.B * a.Hk * a.groups * a.fars;
+        far = id < nfar;
+        if (far) {
+            slot = id * 32 * nw;
+            slices = a.fars;
             slice = (int)(id % slices);
             id /= slices;
-            tile = (int)(id % a.nst);
-            bh = (int)(id / a.nst);
+            k0 = (int)(id % a.groups) * 32;
+            bh = (int)(id / a.groups);
         } else {
-            id -= nsink;
-            slices = a.snorm;
-            slot = slices > 1 ? (a.ssink > 1 ? nsink : 0) + id : -1;
+            id -= nfar;
+            const long at = id;
+            slices = a.slices;
             slice = (int)(id % slices);
             id /= slices;
-            tile = a.nst + (int)(id % (a.nkt - a.nst));
-            bh = (int)(id / (a.nkt - a.nst));
+            const int tile = (int)(id % a.nkt);
+            k0 = tile * kb;
+            bh = (int)(id / a.nkt);
+            slot = slices > 1 ? at : a.groups > 0 && tile < a.nst ? (long)bh * a.nst + tile : -1;
+            if (slot >= 0) slot = nfar * 32 * nw + slot * kb;
         }
     }
 };
 
-template <typename T, int DT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_kernel(const BwdArgs a)
+template <typename T, int DT, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_kernel(const BwdArgs a)
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
-    constexpr int TB = RT * L::RB, BUF = 2 * TB + 3 * RT * 4;
+    constexpr int KB = 32 * NW, RT = row_tile<T, DT>(), TB = RT * L::RB, BUF = 2 * TB + 3 * RT * 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][Q tile, dO tile, lse, delta, position]
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
-    const KeyTile kt(a, xcd_item(blockIdx.x, gridDim.x));
-    const int b = kt.bh / a.Hk, hk = kt.bh - b * a.Hk;
+    const Walk w(a, xcd_item(blockIdx.x, gridDim.x), KB, NW);
+    const int b = w.bh / a.Hk, hk = w.bh - b * a.Hk;
     const int len = a.view.len(b), start = a.view.first(b);
-    const int k0 = kt.tile * KB, k1 = min(k0 + KB, len) - 1;
 
-    // rows that see any of these keys: positions k0 - right .. k1 + left, or to the end where first tokens are among the keys
+    // rows that see the tile's keys k0 .. k1 in their window: positions k0 - right .. k1 + left; behind them the far rows of first tokens
     int ra = 0, rb = 0;
-    if (k0 <= k1) {
-        const int last = min(a.N - 1, len - 1 - start), ia = max(k0 - a.view.right - start, 0);
-        const int ib = k0 < a.view.sinks ? last : min(last, k1 + a.view.left - start);
-        if (ia <= ib) {
+    {
+        const int k0 = w.k0 / KB * KB, k1 = min(k0 + KB, len) - 1;
+        const int last = min(a.N - 1, len - 1 - start), ib = k1 + a.view.left - start;
+        const int ia = max(w.far ? ib + 1 : k0 - a.view.right - start, 0), iz = w.far ? last : min(last, ib);
+        if (k0 <= k1 && ia <= iz) {
             ra = ia * a.G;
-            rb = (ib + 1) * a.G;
+            rb = (iz + 1) * a.G;
         }
     }
     const int all = (rb - ra + a.rt - 1) / a.rt;
-    const int t0 = (int)((long)all * kt.slice / kt.slices), t1 = (int)((long)all * (kt.slice + 1) / kt.slices);
+    const int t0 = (int)((long)all * w.slice / w.slices), t1 = (int)((long)all * (w.slice + 1) / w.slices);
 
-    const int wk = __builtin_amdgcn_readfirstlane(k0 + wave * 32), wk1 = min(wk + 31, len - 1);
+    const int wk = __builtin_amdgcn_readfirstlane(w.far ? w.k0 : w.k0 + wave * 32), wk1 = min(wk + 31, len - 1);
     const bool wave_on = wk < len;
     const int j = wk + (l & 31);
     // this lane's key is seen from positions plo .. plo + span
@@ -206,11 +213,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_k
 
     // A tile is a.rt rows: whole queries, so that a thread's rows have the same head and the same distance from the tile's first query every time.
     // (More than RT heads a group: RT rows from anywhere, decoded each time.)
-    Stage<T, DT, RT> sq, sg;
+    Stage<T, DT, RT, 64 * NW> sq, sg;
     const bool whole = a.G <= RT;
     float pl = 0.f, pd = 0.f;
     int pp = 0;
-    const T *qp = (const T *)a.q + b * a.qb + hk * a.G * a.qh, *gp = (const T *)a.dout + b * a.gb + hk * a.G * a.gh;
+    const T *qp = (const T *)a.q + b * a.qb + (long)hk * a.G * a.qh, *gp = (const T *)a.dout + b * a.gb + (long)hk * a.G * a.gh;
     auto place = [&](int first) {                              // offsets of the tile's rows from query first / G
 #pragma unroll
         for (int u = 0; u < sq.N; ++u) {
@@ -261,7 +268,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_k
 #pragma unroll
         for (int sub = 0; sub < RT / 32; ++sub) {
             const int rs = ra + t * a.rt + sub * 32, re = min(min(rs + 31, ra + t * a.rt + a.rt - 1), rb - 1);
-            if (rs > re) continue;
+            if (rs > re || (w.far && (t * (RT / 32) + sub) % NW != wave)) continue;
             const int p0 = start + a.g.div(rs), p1 = start + a.g.div(re);
             if (!(p1 >= wk - a.view.right && (p0 <= wk1 + a.view.left || wk < a.view.sinks))) continue;
             pa_f16v s = (pa_f16v)(0.f), dp = (pa_f16v)(0.f);
@@ -296,8 +303,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_k
             }
         }
     }
-    if (kt.slot >= 0) {
-        float *po = a.part + ((size_t)kt.slot * KB + wave * 32 + (l & 31)) * (2 * DT);
+    if (w.slot >= 0) {
+        float *po = a.part + ((size_t)w.slot + wave * 32 + (l & 31)) * (2 * DT);
 #pragma unroll
         for (int ct = 0; ct < DT / 32; ++ct)
 #pragma unroll
@@ -324,21 +331,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_k
         }
 }
 
-// dk, dv of the sliced key tiles: the slices' partial sums in their order.  One workgroup per tile and 16 keys.
-template <typename T, int DT>
-__global__ __launch_bounds__(256) void dkv_join_kernel(const BwdArgs a, int first, int tiles, int slices, long slot0)
+// dk, dv of the key tiles that left partial sums: the window's slices in their order, then the far rows' (slice by slice, wave by wave).  A thread owns
+// four elements of dk or dv of a key.
+template <typename T, int DT, int NW>
+__global__ __launch_bounds__(256) void dkv_join_kernel(const BwdArgs a, int tiles)
 {
-    constexpr int C = DT / 2;                                  // threads of a key: dk and dv, four elements each
+    constexpr int C = DT / 2, KB = 32 * NW;
     const long id = ((long)blockIdx.x * 256 + threadIdx.x) / C;
     const int c = (int)(((long)blockIdx.x * 256 + threadIdx.x) % C) * 4;
     const long tile = id / KB;
     const int r = (int)(id % KB);
     if (tile >= (long)a.B * a.Hk * tiles) return;
-    const int bh = (int)(tile / tiles), t = first + (int)(tile % tiles), b = bh / a.Hk, hk = bh - b * a.Hk, j = t * KB + r;
+    const int bh = (int)(tile / tiles), t = (int)(tile % tiles), b = bh / a.Hk, hk = bh - b * a.Hk, j = t * KB + r;
     if (j >= a.view.m) return;
-    const float *p = a.part + ((size_t)(slot0 + tile * slices) * KB + r) * (2 * DT) + c;
+    const size_t nfar = (size_t)a.B * a.Hk * a.groups * a.fars * 32 * NW;
+    const float *p = a.part + (nfar + (size_t)tile * a.slices * KB + r) * (2 * DT) + c;
     pa_f4 s = (pa_f4)(0.f);
-    for (int i = 0; i < slices; ++i) s += *reinterpret_cast<const pa_f4 *>(p + (size_t)i * KB * 2 * DT);
+    for (int i = 0; i < a.slices; ++i) s += *reinterpret_cast<const pa_f4 *>(p + (size_t)i * KB * 2 * DT);
+    if (j / 32 < a.groups) {
+        p = a.part + (((size_t)bh * a.groups + j / 32) * a.fars * 32 * NW + (j & 31)) * (2 * DT) + c;
+        for (int i = 0; i < a.fars * NW; ++i) s += *reinterpret_cast<const pa_f4 *>(p + (size_t)i * 32 * 2 * DT);
+    }
     const size_t at = (((size_t)b * a.view.m + j) * a.Hk + hk) * a.D;
     if (c < DT) {
         if (c < a.D) st4<T>((T *)a.dk + at + c, s[0] * a.scale, s[1] * a.scale, s[2] * a.scale, s[3] * a.scale);
@@ -347,45 +360,70 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(const BwdArgs a, int firs
     }
 }
 
-struct Slices {
-    int nst, nkt, ssink, snorm;
+struct Shape {
+    int qwaves, nqt, kwaves, nkt, slices, nst, groups, fars, rt;
+    long slots(long bh) const                                  // keys of partial sums
+    {
+        return bh * groups * fars * 32 * kwaves + (slices > 1 ? bh * nkt * slices : groups > 0 ? bh * nst : 0) * 32 * kwaves;
+    }
+    int joined() const { return slices > 1 ? nkt : groups > 0 ? nst : 0; }      // key tiles with partial sums
 };
 
-// Slices of a key tile's walk.  Keys that do not fill the chip (fewer than 512 workgroups) have their walks cut, each slice with at least four row
-// tiles; the tiles of first tokens are cut into as many slices as make theirs no longer than the others'.
-Slices slices_of(int B, int N, int M, int H, int Hk, int left, int right, int sinks)
+// Slices: keys that do not fill the chip (fewer than 2048 waves, two per SIMD) have their walks cut, each slice with at least four row tiles; far rows into slices of
+// twice as many row tiles, on each of which one wave works.
+Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int right, int sinks, bool started)
 {
-    Slices s;
-    const long G = H / Hk;
-    s.nkt = pa_div_up(M, KB);
-    const long sk = sinks < M ? sinks : M;
-    s.nst = pa_div_up(sk, KB);
-    const long wgs = (long)B * Hk * s.nkt, reach = (long)left + right + KB, rt = G <= RT ? RT / G * G : RT, walk = pa_div_up((N < reach ? N : reach) * G, rt), whole = pa_div_up(N * G, rt);
-    long n = wgs ? 512 / wgs : 1;
+    Shape s;
+    const long G = H / Hk, bh = (long)B * Hk, rows = (long)N * G;
+    s.qwaves = waves_of(bh * ((rows + 127) / 128));
+    s.nqt = pa_div_up(rows, 32 * s.qwaves);
+    s.kwaves = waves_of(bh * ((M + 127l) / 128));
+    const int kb = 32 * s.kwaves, rt = width(d) * es >= 512 ? 32 : 64;
+    s.rt = G <= rt ? rt / (int)G * (int)G : rt;
+    s.nkt = pa_div_up(M, kb);
+    const long wgs = bh * s.nkt, reach = (long)left + right + kb, walk = pa_div_up((N < reach ? N : reach) * G, s.rt);
+    long n = wgs ? 2048 / s.kwaves / wgs : 1;
     if (n > walk / 4) n = walk / 4;
-    s.snorm = n < 1 ? 1 : n > 64 ? 64 : (int)n;
-    long per = pa_div_up(walk, s.snorm);                        // row tiles of one slice
-    if (per < 4) per = 4;
-    long m = pa_div_up(whole, per);
-    s.ssink = s.nst == 0 || m < 1 ? 1 : m > 256 ? 256 : (int)m;
+    s.slices = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+    const int first = sinks < M ? sinks : M;
+    const bool far = first > 0 && (started ? left < M : left < N - 1);          // rows behind the window of the first tokens
+    s.groups = far ? pa_div_up(first, 32) : 0;
+    s.nst = pa_div_up(first, kb);
+    const long per = (walk + s.slices - 1) / s.slices;                          // row tiles of a slice
+    const long f = pa_div_up(rows, s.rt) / (2 * per > 8 ? 2 * per : 8) + 1;
+    s.fars = far ? (f > 64 ? 64 : (int)f) : 1;
     return s;
 }
 
-template <typename T, int DT>
-int launch_bwd(const BwdArgs &a, hipStream_t st)
+template <typename T, int DT, int NW>
+void launch_dq(const BwdArgs &a, hipStream_t st)
 {
-    constexpr int lq = 4 * KT * DT * (int)sizeof(T), lk = 2 * (2 * RT * DT * (int)sizeof(T) + 3 * RT * 4);
-    if (lq > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&dq_kernel<T, DT>), hipFuncAttributeMaxDynamicSharedMemorySize, lq);
-    if (lk > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&dkv_kernel<T, DT>), hipFuncAttributeMaxDynamicSharedMemorySize, lk);
-    if (a.nqt) hipLaunchKernelGGL((dq_kernel<T, DT>), dim3((unsigned)((long)a.nqt * a.B * a.Hk)), dim3(256), lq, st, a);
-    const long bh = (long)a.B * a.Hk, sink = bh * a.nst * a.ssink, norm = bh * (a.nkt - a.nst) * a.snorm;
-    if (sink + norm == 0) return 0;
-    hipLaunchKernelGGL((dkv_kernel<T, DT>), dim3((unsigned)(sink + norm)), dim3(256), lk, st, a);
-    if (a.ssink > 1 && a.nst > 0)
-        hipLaunchKernelGGL((dkv_join_kernel<T, DT>), dim3((unsigned)(bh * a.nst * KB * (DT / 2) / 256)), dim3(256), 0, st, a, 0, a.nst, a.ssink, 0l);
-    if (a.snorm > 1 && a.nkt > a.nst)
-        hipLaunchKernelGGL((dkv_join_kernel<T, DT>), dim3((unsigned)(bh * (a.nkt - a.nst) * KB * (DT / 2) / 256)), dim3(256), 0, st, a, a.nst, a.nkt - a.nst, a.snorm,
-                           a.ssink > 1 ? sink : 0l);
+    constexpr int lds = 4 * key_tile<T, DT, NW>() * DT * (int)sizeof(T);
+    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&dq_kernel<T, DT, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipLaunchKernelGGL((dq_kernel<T, DT, NW>), dim3((unsigned)((long)a.nqt * a.B * a.Hk)), dim3(64 * NW), lds, st, a);
+}
+
+template <typename T, int DT, int NW>
+void launch_dkv(const BwdArgs &a, int joined, hipStream_t st)
+{
+    constexpr int RT = row_tile<T, DT>(), lds = 2 * (2 * RT * DT * (int)sizeof(T) + 3 * RT * 4);
+    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&dkv_kernel<T, DT, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    const long bh = (long)a.B * a.Hk;
+    hipLaunchKernelGGL((dkv_kernel<T, DT, NW>), dim3((unsigned)(bh * a.groups * a.fars + bh * a.nkt * a.slices)), dim3(64 * NW), lds, st, a);
+    if (joined) hipLaunchKernelGGL((dkv_join_kernel<T, DT, NW>), dim3((unsigned)(bh * joined * 32 * NW * (DT / 2) / 256)), dim3(256), 0, st, a, joined);
+}
+
+template <typename T, int DT>
+int launch_bwd(const BwdArgs &a, const Shape &s, hipStream_t st)
+{
+    if (a.nqt) {
+        if (s.qwaves == 2) launch_dq<T, DT, 2>(a, st);
+        else launch_dq<T, DT, 4>(a, st);
+    }
+    if (a.nkt) {
+        if (s.kwaves == 2) launch_dkv<T, DT, 2>(a, s.joined(), st);
+        else launch_dkv<T, DT, 4>(a, s.joined(), st);
+    }
     return 0;
 }
 
@@ -395,9 +433,13 @@ int launch_bwd(const BwdArgs &a, hipStream_t st)
 PA_API long pa_window_attention_backward_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks)
 {
     if (b <= 0 || n <= 0 || h <= 0 || hk <= 0 || h % hk != 0 || m < 0 || sinks < 0) return 0;
-    const Slices s = slices_of(b, n, m, h, hk, left < 0 ? UNBOUNDED : left, right < 0 ? UNBOUNDED : right, sinks);
-    const long bh = (long)b * hk, slots = (s.ssink > 1 ? bh * s.nst * s.ssink : 0) + (s.snorm > 1 ? bh * (s.nkt - s.nst) * s.snorm : 0);
-    return pa_div_up((long)b * h * n, 4) * 4l + slots * KB * 2 * width(d);
+    const long bh = (long)b * hk;
+    long most = 0;                                              // of both element sizes, with and without q_start
+    for (int i = 0; i < 4; ++i) {
+        const long k = shape_of(b, n, m, h, hk, d, i & 1 ? 4 : 2, left < 0 ? UNBOUNDED : left, right < 0 ? UNBOUNDED : right, sinks, i & 2).slots(bh);
+        most = k > most ? k : most;
+    }
+    return pa_div_up((long)b * h * n, 4) * 4l + most * 2 * width(d);
 }
 
 PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb,
@@ -420,18 +462,16 @@ PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, i
     a.scale = scale;
     a.c = scale * 1.4426950408889634f;
     a.g = Div(a.G);
-    a.nqt = pa_div_up((long)n * a.G, QT);
-    const Slices s = slices_of(b, n, m, h, hk, a.view.left, a.view.right, sinks);
-    a.rt = a.G <= RT ? RT / a.G * a.G : RT;
-    a.nst = s.nst; a.nkt = s.nkt; a.ssink = s.ssink; a.snorm = s.snorm;
+    const Shape s = shape_of(b, n, m, h, hk, d, dtype == PA_DT_F32 ? 4 : 2, a.view.left, a.view.right, sinks, start != nullptr);
+    a.nqt = s.nqt; a.nkt = s.nkt; a.slices = s.slices; a.nst = s.nst; a.groups = s.groups; a.fars = s.fars; a.rt = s.rt;
     PA_REQUIRE(kn >= 0 && vn >= 0 && kn <= PA_ATTN_MAXSTRIDE && vn <= PA_ATTN_MAXSTRIDE && qn >= 0 && qh >= 0 && gn >= 0 && gh >= 0 && qn <= PA_ATTN_MAXSTRIDE &&
                    gn <= PA_ATTN_MAXSTRIDE && qh <= PA_ATTN_MAXSTRIDE && gh <= PA_ATTN_MAXSTRIDE,
                "pa_window_attention_backward: tokens or heads are more than 2^22 elements apart");
-    PA_REQUIRE(a.G <= RT || (long)a.G * (qh > gh ? qh : gh) * 4 < (1l << 31), "pa_window_attention_backward: the heads of a group span 2^31 bytes");
-    PA_REQUIRE((long)a.nqt * b * hk < (1l << 31) && (long)b * hk * ((long)s.nst * s.ssink + (long)(s.nkt - s.nst) * s.snorm) * 32 < (1l << 31),
+    PA_REQUIRE(a.G <= 32 || (long)a.G * (qh > gh ? qh : gh) * 4 < (1l << 31), "pa_window_attention_backward: the heads of a group span 2^31 bytes");
+    PA_REQUIRE((long)a.nqt * b * hk < (1l << 31) && (long)b * hk * ((long)s.groups * s.fars + (long)s.nkt * s.slices) * 128 < (1l << 31),
                "pa_window_attention_backward: too many workgroups");
     hipStream_t st = (hipStream_t)stream;
-#define BWD(T, DT) launch_bwd<T, DT>(a, st)
+#define BWD(T, DT) launch_bwd<T, DT>(a, s, st)
     PA_ATTN_DISPATCH(dtype, d, BWD);
 #undef BWD
     PA_CHECK_LAUNCH("pa_window_attention_backward");
