@@ -14,6 +14,8 @@ Types: float32, float16, bfloat16 (sums, soft-max and norms in 32 bits).  Heads:
 ``i`` reads key head ``i // (H // Hk)``.  Everything runs on the current stream of the tensors' device through libpatchaugnet_hip.so; there is no
 CPU form.
 """
+import contextlib
+import functools
 import math
 
 import torch
@@ -21,13 +23,14 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, ptr
+from ._lib import call
 
 __all__ = ["qk_norm_rotary", "window_attention", "paged_append", "paged_attention"]
 
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _FAR = 1 << 22             # elements between neighbouring tokens or heads: 32-bit offsets inside a tile (pa_attn.h)
 _PTYPE = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_HERE = contextlib.nullcontext()
 _MAXLEN = 1 << 28            # tokens of a sequence (pa_attn.h)
 
 
@@ -39,18 +42,26 @@ def _check(name, *tensors):
             raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
         if not t.is_cuda:
             raise RuntimeError(f"{name} runs on the MI355X only: got a tensor on {t.device} (there is no CPU form)")
-        if t.dtype != first.dtype or t.dtype not in _DTYPE:
-            raise TypeError(f"{name}: tensors of one type out of float32, float16, bfloat16; got {[x.dtype for x in tensors]}")
+        if t.dtype != first.dtype:
+            raise TypeError(f"{name}: tensors of one type; got {[x.dtype for x in tensors]}")
         if t.device != first.device:
             raise RuntimeError(f"{name}: tensors on {first.device} and {t.device}")
-    return _DTYPE[first.dtype]
+    dt = _DTYPE.get(first.dtype)
+    if dt is None:
+        raise TypeError(f"{name}: float32, float16 or bfloat16; got {first.dtype}")
+    return dt
+
+
+def _on(device):
+    """The device's context; nothing where it is current already (entering costs as much as a launch)."""
+    return _HERE if _lib._cur_device is not None and device.index == _lib._cur_device() else torch.cuda.device(device)
 
 
 def _ints(name, what, t, device, n):
     """A (n,) int32 device vector or None."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or tuple(t.shape) != (n,):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name}: {what} has to be an int32 tensor of shape ({n},) on {device}")
     return t.contiguous()
 
@@ -58,16 +69,32 @@ def _ints(name, what, t, device, n):
 def _rows(t, align=16, far=1 << 62):
     """t itself if its last dimension is contiguous, every row starts at a multiple of `align` bytes and those of neighbouring tokens and heads lie at most
     `far` elements apart, else a contiguous copy."""
-    es = t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % align == 0 and all(s * es % align == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1) \
-            and all(s <= far for s, n in zip(t.stride()[1:-1], t.shape[1:-1]) if n > 1) and (far > _FAR or t.shape[-2] * t.stride(-2) * 4 < 1 << 31):
+    if t.is_contiguous():
+        return t if t.data_ptr() % align == 0 else t.clone()
+    s = t.stride()
+    outer, es = 0, t.element_size()
+    for i, n in zip(s[:-1], t.shape):
+        if n > 1:
+            outer |= i
+    if s[-1] == 1 and t.data_ptr() % align == 0 and outer * es % align == 0 and (far > _FAR or _near(t, s)):
         return t
     return t.contiguous()
 
 
+def _near(t, s):
+    return all(i <= _FAR for i, n in zip(s[1:-1], t.shape[1:-1]) if n > 1) and t.shape[-2] * s[-2] * 4 < 1 << 31
+
+
+def _unit(t):
+    """t itself if its last dimension is contiguous, else a contiguous copy."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
 def _strides(t):
     """Strides of all dimensions but the last; 0 where a dimension has one entry (its stride is never used and may be anything)."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+    if t.is_contiguous():
+        return t.stride()[:-1]
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
 
 
 def _side(name, what, n):
@@ -92,6 +119,16 @@ def _scale(name, scale, D):
     return s
 
 
+def ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+@functools.lru_cache(maxsize=256)
+def _size(name, *sizes):
+    """Floats of scratch that the library asks for at these sizes."""
+    return getattr(_lib.lib(), name)(*sizes)
+
+
 def _floats(n, device):
     return torch.empty(n, dtype=torch.float32, device=device) if n else None
 
@@ -106,13 +143,17 @@ def _norm_args(dt, q, k, qw, kw, pos, freq, eps, interleaved):
     return head + place + (eps, interleaved)
 
 
+def _norm_forward(q, k, qw, kw, pos, freq, eps, interleaved):
+    out = q.new_empty(q.shape), k.new_empty(k.shape)
+    with _on(q.device):
+        call("pa_qk_norm_rotary", *_norm_args(_DTYPE[q.dtype], q, k, qw, kw, pos, freq, eps, interleaved), ptr(out[0]), ptr(out[1]))
+    return out
+
+
 class _NormRotary(Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, pos, freq, eps, interleaved):
-        q, k = _rows(q, q.element_size()), _rows(k, k.element_size())
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        with torch.cuda.device(q.device):
-            call("pa_qk_norm_rotary", *_norm_args(_DTYPE[q.dtype], q, k, qw, kw, pos, freq, eps, interleaved), ptr(out[0]), ptr(out[1]))
+        out = _norm_forward(q, k, qw, kw, pos, freq, eps, interleaved)
         ctx.save_for_backward(q, k, qw, kw, pos, freq)
         ctx.rest = eps, interleaved
         return out
@@ -122,16 +163,16 @@ class _NormRotary(Function):
     def backward(ctx, gq, gk):
         q, k, qw, kw, pos, freq = ctx.saved_tensors
         D = q.shape[3]
-        gq, gk = _rows(gq, gq.element_size()), _rows(gk, gk.element_size())
-        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        with torch.cuda.device(q.device):
+        gq, gk = _unit(gq), _unit(gk)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+        with _on(q.device):
             empty = q.shape[0] * q.shape[1] == 0
             make = torch.zeros if empty else torch.empty
             dqw = make(D, dtype=torch.float32, device=q.device) if ctx.needs_input_grad[2] else None
             dkw = make(D, dtype=torch.float32, device=q.device) if ctx.needs_input_grad[3] else None
             scratch = None
             if dqw is not None or dkw is not None:
-                scratch = _floats(_lib.lib().pa_qk_norm_rotary_backward_scratch_floats(q.shape[0], q.shape[1], D), q.device)
+                scratch = _floats(_size("pa_qk_norm_rotary_backward_scratch_floats", q.shape[0], q.shape[1], D), q.device)
             call("pa_qk_norm_rotary_backward", *_norm_args(_DTYPE[q.dtype], q, k, qw, kw, pos, freq, *ctx.rest), ptr(gq), *_strides(gq), ptr(gk), *_strides(gk),
                  ptr(dq), ptr(dk), ptr(dqw), ptr(dkw), ptr(scratch))
         cast = [None if g is None else g.to(w.dtype) for g, w in ((dqw, qw), (dkw, kw))]
@@ -181,7 +222,11 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, *, positions=None, inv_fr
         elif shape not in ((N, A), (B, N, A)):
             raise ValueError(f"{name}: positions of shape {shape} fit neither (N, A) = ({N}, {A}) nor (B, N, A) with B = {B}")
         positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    return _NormRotary.apply(q, k, *(w.contiguous() if w is not None else None for w in (q_weight, k_weight)), positions, inv_freq, float(eps), int(bool(interleaved)))
+    q, k = _unit(q), _unit(k)
+    qw, kw = (w.contiguous() if w is not None else None for w in (q_weight, k_weight))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any(w.requires_grad for w in ws)):
+        return _NormRotary.apply(q, k, qw, kw, positions, inv_freq, float(eps), int(bool(interleaved)))
+    return _norm_forward(q, k, qw, kw, positions, inv_freq, float(eps), int(bool(interleaved)))
 
 
 # ------------------------------------------------------------------------------------------------------------------- window attention
@@ -190,12 +235,12 @@ def _window_sizes(q, k, view):
 
 
 def _window_forward(q, k, v, start, length, view, want_lse):
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     B, N, H, D = q.shape
     lse = torch.empty((B, H, N), dtype=torch.float32, device=q.device) if want_lse else None
     left, right, sinks, scale = view
-    with torch.cuda.device(q.device):
-        scratch = _floats(_lib.lib().pa_window_attention_scratch_floats(*_window_sizes(q, k, view)), q.device)
+    with _on(q.device):
+        scratch = _floats(_size("pa_window_attention_scratch_floats", *_window_sizes(q, k, view)), q.device)
         call("pa_window_attention", _DTYPE[q.dtype], B, N, k.shape[1], H, k.shape[2], D, ptr(q), *_strides(q), ptr(k), *_strides(k), ptr(v), *_strides(v),
              left, right, sinks, scale, ptr(start), ptr(length), ptr(out), ptr(lse), ptr(scratch))
     return out, lse
@@ -215,10 +260,10 @@ class _WindowAttention(Function):
         q, k, v, start, length, out, lse = ctx.saved_tensors
         g = _rows(g, far=_FAR)
         left, right, sinks, scale = ctx.view
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
         B, N, H, D = q.shape
-        with torch.cuda.device(q.device):
-            scratch = _floats(_lib.lib().pa_window_attention_backward_scratch_floats(*_window_sizes(q, k, ctx.view)), q.device)
+        with _on(q.device):
+            scratch = _floats(_size("pa_window_attention_backward_scratch_floats", *_window_sizes(q, k, ctx.view)), q.device)
             call("pa_window_attention_backward", _DTYPE[q.dtype], B, N, k.shape[1], H, k.shape[2], D, ptr(q), *_strides(q), ptr(k), *_strides(k), ptr(v),
                  *_strides(v), ptr(out), ptr(lse), ptr(g), *_strides(g), left, right, sinks, scale, ptr(start), ptr(length), ptr(dq), ptr(dk), ptr(dv),
                  ptr(scratch))
@@ -256,7 +301,7 @@ def _cache(name, k_pages, v_pages, table, B):
     if k_pages.shape[1] < 1 or k_pages.shape[2] < 1:
         raise ValueError(f"{name}: empty pages or no key heads: {tuple(k_pages.shape)}")
     for t in (k_pages, v_pages):
-        if _rows(t) is not t:
+        if _rows(t) is not t and t.numel():
             raise ValueError(f"{name}: a row of a page has to be contiguous and to start at a multiple of 16 bytes")
     if not isinstance(table, torch.Tensor) or table.dtype != torch.int32 or table.device != k_pages.device or table.dim() != 2 or table.shape[0] != B:
         raise ValueError(f"{name}: page_table has to be an int32 tensor (B, pages of a sequence) on {k_pages.device}, B = {B}")
@@ -288,7 +333,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, starts, *, counts=None):
         raise ValueError(f"{name}: starts are needed")
     starts, counts = _ints(name, "starts", starts, k.device, B), _ints(name, "counts", counts, k.device, B)
     k, v = _rows(k), _rows(v)
-    with torch.cuda.device(k.device):
+    with _on(k.device):
         call("pa_paged_append", dt, B, T, Hk, D, ptr(k), *_strides(k), ptr(v), *_strides(v), ptr(k_pages), *_strides(k_pages), ptr(v_pages), *_strides(v_pages),
              k_pages.shape[0], k_pages.shape[1], ptr(table), table.shape[1], ptr(starts), ptr(counts))
 
@@ -314,9 +359,9 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, left=None, sink
     left, sinks = _side(name, "left", left), max(_side(name, "sinks", sinks), 0)
     scale = _scale(name, scale, D)
     q = _rows(q)
-    out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
-    with torch.cuda.device(q.device):
-        scratch = _floats(_lib.lib().pa_paged_attention_scratch_floats(B, H, Hk, D, page, table.shape[1], left, sinks), q.device)
+    out = q.new_empty(q.shape)
+    with _on(q.device):
+        scratch = _floats(_size("pa_paged_attention_scratch_floats", B, H, Hk, D, page, table.shape[1], left, sinks), q.device)
         call("pa_paged_attention", dt, B, H, Hk, D, ptr(q), *_strides(q), ptr(k_pages), *_strides(k_pages), ptr(v_pages), *_strides(v_pages), P, page, ptr(table),
              table.shape[1], ptr(lengths), left, sinks, scale, ptr(out), ptr(scratch))
     return out

@@ -15,25 +15,34 @@
 // second launch over the workgroups' rows, always in the same order.
 #include <initializer_list>
 
-#include "pa_common.h"
+#include "pa_attn.h"
+
+using pa_attn::Div;
 
 namespace {
 
-enum { F32 = 0, F16 = 1, BF16 = 2 };
+enum { F32 = PA_DT_F32, F16 = PA_DT_F16, BF16 = PA_DT_BF16 };
 constexpr int MAXD = 512, MAXTOK = 16;
+constexpr int MAXGROUPS = 768;         // workgroups of the backward pass: three per CU are resident at its registers, one round
+
+struct Side {                           // the queries, or the keys
+    const void *x, *g, *w;              // input, gradient of the output (backward), weights
+    void *y;                            // output (forward) / input gradient (backward), contiguous
+    long xb, xn, xh, gb, gn, gh;
+    int heads;
+    Div d;
+};
 
 struct NormArgs {
-    const void *q, *k, *gq, *gk;        // gq, gk: gradients of the outputs (backward)
-    void *oq, *ok;                      // outputs (forward) / input gradients (backward), contiguous
-    const void *qw, *kw;
+    Side side[2];
     const void *pos;
     const float *freq;
     float *part;                        // (workgroups, 2, D) partial weight gradients
-    long qb, qn, qh, kb, kn, kh, gqb, gqn, gqh, gkb, gkn, gkh, pb;
-    long tokens;
-    int N, H, Hk, D, axes, per, pairs, interleaved, wtype, ptype;
+    long pb;
+    int tokens, N, D, axes, per, pairs, interleaved, wtype, ptype;
     int tb, units, lpr;                 // tokens of a workgroup's turn, units of a row, lanes of a row (a power of two)
     float eps;
+    Div dn, dpairs, dper;
 };
 
 template <typename T> __device__ __forceinline__ float weight_at(const void *w, int f32, int i)
@@ -62,25 +71,19 @@ __device__ __forceinline__ float2 turn(double x)
 
 template <typename T, int V> struct Vec {
     typedef T type __attribute__((ext_vector_type(V)));
+    __device__ static __forceinline__ float get(const type &v, int i) { return (float)v[i]; }
+    __device__ static __forceinline__ void set(type &v, int i, float x) { v[i] = (T)x; }
 };
 template <typename T> struct Vec<T, 1> {
     typedef T type;
+    __device__ static __forceinline__ float get(const type &v, int) { return (float)v; }
+    __device__ static __forceinline__ void set(type &v, int, float x) { v = (T)x; }
 };
-template <typename T, int V> __device__ __forceinline__ void load(float *x, const T *p)
-{
-    const typename Vec<T, V>::type v = *reinterpret_cast<const typename Vec<T, V>::type *>(p);
-    if constexpr (V == 1) x[0] = (float)v;
-    else
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = (float)v[i];
-}
 template <typename T, int V> __device__ __forceinline__ void store(T *p, const float *x)
 {
     typename Vec<T, V>::type v;
-    if constexpr (V == 1) v = (T)x[0];
-    else
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (T)x[i];
+    for (int i = 0; i < V; ++i) Vec<T, V>::set(v, i, x[i]);
     *reinterpret_cast<typename Vec<T, V>::type *>(p) = v;
 }
 
@@ -125,14 +128,110 @@ template <int V> __device__ __forceinline__ void rotate(float *x, const Unit<V> 
     }
 }
 
+// 1 / sqrt(x): v_rsq_f32 and a Newton step; it flushes subnormal arguments, so small ones are lifted first
+__device__ __forceinline__ float rsqrt32(float x)
+{
+    const bool low = x < 0x1p-100f;
+    x = low ? x * 0x1p100f : x;
+    float r = __builtin_amdgcn_rsqf(x);
+    r = r * __builtin_fmaf(-0.5f * x * r, r, 1.5f);
+    return low ? r * 0x1p50f : r;
+}
+
+// The rows of one side in a workgroup's turn of nt tokens from t0: row slot by row slot, the next one fetched while this one is computed.  where:
+// offsets of the turn's tokens in x and in g; cos, sin: their angles.  acc: this lane's sums for the weights' gradient.
+template <typename T, int V, int UPL, bool BWD>
+__device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int t0, int nt, const long *where, const float *cos, const float *sin,
+                                          const float (&w)[UPL][2 * V], float (&acc)[BWD ? UPL : 1][2 * V])
+{
+    typedef typename Vec<T, V>::type P;
+    const int tid = threadIdx.x, lane = tid & (a.lpr - 1), slot = tid / a.lpr, slots = 256 / a.lpr, rows = nt * sd.heads;
+    const float inv_d = 1.0f / (float)a.D;
+    struct Row {
+        P x[UPL][2], g[BWD ? UPL : 1][2];
+        T *y;
+        int tok;
+    } cur, nxt;
+    auto fetch = [&](Row &r, int row) {
+        r.tok = sd.d.div(row);
+        const int hd = row - r.tok * sd.heads;
+        const T *x = (const T *)sd.x + where[r.tok] + hd * sd.xh, *dy = BWD ? (const T *)sd.g + where[MAXTOK + r.tok] + hd * sd.gh : nullptr;
+        r.y = (T *)sd.y + ((long)t0 * sd.heads + row) * a.D;
+#pragma unroll
+        for (int p = 0; p < UPL; ++p) {
+            const Unit<V> t(a, lane + p * a.lpr);
+            r.x[p][0] = r.x[p][1] = 0;
+            if (t.on) r.x[p][0] = *reinterpret_cast<const P *>(x + t.o1);
+            if (t.two) r.x[p][1] = *reinterpret_cast<const P *>(x + t.o2);
+            if (BWD) {
+                r.g[p][0] = r.g[p][1] = 0;
+                if (t.on) r.g[p][0] = *reinterpret_cast<const P *>(dy + t.o1);
+                if (t.two) r.g[p][1] = *reinterpret_cast<const P *>(dy + t.o2);
+            }
+        }
+    };
+    if (slot < rows) fetch(cur, slot);
+    for (int row = slot; row < rows; row += slots) {
+        if (row + slots < rows) fetch(nxt, row + slots);
+        float v[UPL][2 * V], gr[BWD ? UPL : 1][2 * V], ss = 0.f;
+        const float *cs = cos + cur.tok * a.pairs, *sn = sin + cur.tok * a.pairs;
+#pragma unroll
+        for (int p = 0; p < UPL; ++p)
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) {
+                v[p][i] = Vec<T, V>::get(cur.x[p][i / V], i % V);
+                if (BWD) gr[p][i] = Vec<T, V>::get(cur.g[p][i / V], i % V);
+                ss = __builtin_fmaf(v[p][i], v[p][i], ss);
+            }
+        for (int o = 1; o < a.lpr; o <<= 1) ss += __shfl_xor(ss, o);
+        const float r = rsqrt32(__builtin_fmaf(ss, inv_d, a.eps));
+        if (!BWD) {
+#pragma unroll
+            for (int p = 0; p < UPL; ++p) {
+                const Unit<V> t(a, lane + p * a.lpr);
+#pragma unroll
+                for (int i = 0; i < 2 * V; ++i) v[p][i] = v[p][i] * r * w[p][i];
+                rotate<V>(v[p], t, a.interleaved, cs, sn, 1.f);
+                if (t.on) store<T, V>(cur.y + t.o1, &v[p][0]);
+                if (t.two) store<T, V>(cur.y + t.o2, &v[p][V]);
+            }
+        } else {
+            float dot = 0.f;
+#pragma unroll
+            for (int p = 0; p < UPL; ++p) {
+                const Unit<V> t(a, lane + p * a.lpr);
+                rotate<V>(gr[p], t, a.interleaved, cs, sn, -1.f);
+#pragma unroll
+                for (int i = 0; i < 2 * V; ++i) {
+                    v[p][i] *= r;                               // n
+                    acc[p][i] = __builtin_fmaf(gr[p][i], v[p][i], acc[p][i]);
+                    gr[p][i] *= w[p][i];
+                    dot = __builtin_fmaf(gr[p][i], v[p][i], dot);
+                }
+            }
+            for (int o = 1; o < a.lpr; o <<= 1) dot += __shfl_xor(dot, o);
+            dot *= inv_d;
+#pragma unroll
+            for (int p = 0; p < UPL; ++p) {
+                const Unit<V> t(a, lane + p * a.lpr);
+#pragma unroll
+                for (int i = 0; i < 2 * V; ++i) gr[p][i] = r * __builtin_fmaf(-v[p][i], dot, gr[p][i]);
+                if (t.on) store<T, V>(cur.y + t.o1, &gr[p][0]);
+                if (t.two) store<T, V>(cur.y + t.o2, &gr[p][V]);
+            }
+        }
+        cur = nxt;
+    }
+}
+
 // UPL: units a lane can hold (1 for the wide pieces, up to 4 for the narrow ones: 64 lanes x 4 units x 2 elements = MAXD)
 template <typename T, int V, int UPL, bool BWD>
-__global__ __launch_bounds__(256) void norm_kernel(const NormArgs a)
+__global__ __launch_bounds__(256, BWD ? 3 : 4) void norm_kernel(const NormArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) float sh[];       // [tb][pairs] cosines, [tb][pairs] sines; backward: then the join of 2 D sums
-    const int tid = threadIdx.x, lane = tid & (a.lpr - 1), slot = tid / a.lpr, slots = 256 / a.lpr;
-    const int heads = a.H + a.Hk;
-    float wq[UPL][2 * V], wk[UPL][2 * V], sq[UPL][2 * V], sk[UPL][2 * V];
+    __shared__ long where[2][2][MAXTOK];
+    const int tid = threadIdx.x, lane = tid & (a.lpr - 1);
+    float w[2][UPL][2 * V], acc[2][BWD ? UPL : 1][2 * V];
 #pragma unroll
     for (int p = 0; p < UPL; ++p) {
         const Unit<V> t(a, lane + p * a.lpr);
@@ -140,95 +239,30 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a)
         for (int i = 0; i < 2 * V; ++i) {
             const int e = (i < V ? t.o1 + i : t.o2 + i - V);
             const bool in = t.on && (i < V || t.two);
-            wq[p][i] = in ? weight_at<T>(a.qw, a.wtype, e) : 0.f;
-            wk[p][i] = in ? weight_at<T>(a.kw, a.wtype, e) : 0.f;
-            sq[p][i] = sk[p][i] = 0.f;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                w[s][p][i] = in ? weight_at<T>(a.side[s].w, a.wtype, e) : 0.f;
+                if (BWD) acc[s][p][i] = 0.f;
+            }
         }
     }
-    const float inv_d = 1.0f / (float)a.D;
-    for (long t0 = (long)blockIdx.x * a.tb; t0 < a.tokens; t0 += (long)gridDim.x * a.tb) {
-        const int nt = (int)(a.tokens - t0 < a.tb ? a.tokens - t0 : a.tb);
-        if (a.pairs > 0) {
-            if (BWD) __syncthreads();                           // readers of the previous turn's angles
-            for (int i = tid; i < nt * a.pairs; i += 256) {
-                const int tok = i / a.pairs, pr = i - tok * a.pairs, axis = pr / a.per;
-                const long at = t0 + tok;
-                const int b = (int)(at / a.N), n = (int)(at - (long)b * a.N);
-                const float2 cs = turn(position_at(a, b, n, axis) * (double)a.freq[pr]);
-                sh[tok * a.pairs + pr] = cs.x;
-                sh[(a.tb + tok) * a.pairs + pr] = cs.y;
-            }
-            __syncthreads();
+    for (int t0 = blockIdx.x * a.tb; t0 < a.tokens; t0 += gridDim.x * a.tb) {
+        const int nt = min(a.tokens - t0, a.tb);
+        if (BWD) __syncthreads();                               // readers of the previous turn's table and angles
+        if (tid < 4 * MAXTOK && (tid & (MAXTOK - 1)) < nt) {
+            const int s = tid / (2 * MAXTOK), g = tid / MAXTOK & 1, tok = tid & (MAXTOK - 1), b = a.dn.div(t0 + tok), n = t0 + tok - b * a.N;
+            const Side &sd = s ? a.side[1] : a.side[0];
+            where[s][g][tok] = g ? b * sd.gb + n * sd.gn : b * sd.xb + n * sd.xn;
         }
-        for (int row = slot; row < nt * heads; row += slots) {
-            const int tok = row / heads, hd = row - tok * heads;
-            const long at = t0 + tok;
-            const int b = (int)(at / a.N), n = (int)(at - (long)b * a.N);
-            const bool isq = hd < a.H;
-            const int g = isq ? hd : hd - a.H;
-            const T *x = isq ? (const T *)a.q + b * a.qb + n * a.qn + g * a.qh : (const T *)a.k + b * a.kb + n * a.kn + g * a.kh;
-            T *y = isq ? (T *)a.oq + (at * a.H + g) * a.D : (T *)a.ok + (at * a.Hk + g) * a.D;
-            float v[UPL][2 * V], gr[BWD ? UPL : 1][2 * V], ss = 0.f;
-            const float *cs = sh + tok * a.pairs, *sn = sh + (a.tb + tok) * a.pairs;
-#pragma unroll
-            for (int p = 0; p < UPL; ++p) {
-                const Unit<V> t(a, lane + p * a.lpr);
-#pragma unroll
-                for (int i = 0; i < 2 * V; ++i) v[p][i] = 0.f;
-                if (t.on) load<T, V>(&v[p][0], x + t.o1);
-                if (t.two) load<T, V>(&v[p][V], x + t.o2);
-                if (BWD) {
-                    const T *gp = isq ? (const T *)a.gq + b * a.gqb + n * a.gqn + g * a.gqh : (const T *)a.gk + b * a.gkb + n * a.gkn + g * a.gkh;
-#pragma unroll
-                    for (int i = 0; i < 2 * V; ++i) gr[p][i] = 0.f;
-                    if (t.on) load<T, V>(&gr[p][0], gp + t.o1);
-                    if (t.two) load<T, V>(&gr[p][V], gp + t.o2);
-                }
-            }
-#pragma unroll
-            for (int p = 0; p < UPL; ++p)
-#pragma unroll
-                for (int i = 0; i < 2 * V; ++i) ss = __builtin_fmaf(v[p][i], v[p][i], ss);
-            for (int o = 1; o < a.lpr; o <<= 1) ss += __shfl_xor(ss, o);
-            const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv_d, a.eps));
-            if (!BWD) {
-#pragma unroll
-                for (int p = 0; p < UPL; ++p) {
-                    const Unit<V> t(a, lane + p * a.lpr);
-#pragma unroll
-                    for (int i = 0; i < 2 * V; ++i) v[p][i] = v[p][i] * r * (isq ? wq[p][i] : wk[p][i]);
-                    rotate<V>(v[p], t, a.interleaved, cs, sn, 1.f);
-                    if (t.on) store<T, V>(y + t.o1, &v[p][0]);
-                    if (t.two) store<T, V>(y + t.o2, &v[p][V]);
-                }
-            } else {
-                float dot = 0.f;
-#pragma unroll
-                for (int p = 0; p < UPL; ++p) {
-                    const Unit<V> t(a, lane + p * a.lpr);
-                    rotate<V>(gr[p], t, a.interleaved, cs, sn, -1.f);
-#pragma unroll
-                    for (int i = 0; i < 2 * V; ++i) {
-                        v[p][i] *= r;                           // n
-                        const float d = gr[p][i] * v[p][i];
-                        sq[p][i] += isq ? d : 0.f;
-                        sk[p][i] += isq ? 0.f : d;
-                        gr[p][i] *= isq ? wq[p][i] : wk[p][i];
-                        dot = __builtin_fmaf(gr[p][i], v[p][i], dot);
-                    }
-                }
-                for (int o = 1; o < a.lpr; o <<= 1) dot += __shfl_xor(dot, o);
-                dot *= inv_d;
-#pragma unroll
-                for (int p = 0; p < UPL; ++p) {
-                    const Unit<V> t(a, lane + p * a.lpr);
-#pragma unroll
-                    for (int i = 0; i < 2 * V; ++i) gr[p][i] = r * (gr[p][i] - v[p][i] * dot);
-                    if (t.on) store<T, V>(y + t.o1, &gr[p][0]);
-                    if (t.two) store<T, V>(y + t.o2, &gr[p][V]);
-                }
-            }
+        for (int i = tid; i < nt * a.pairs; i += 256) {
+            const int tok = a.dpairs.div(i), pr = i - tok * a.pairs, at = t0 + tok, b = a.dn.div(at);
+            const float2 cs = turn(position_at(a, b, at - b * a.N, a.dper.div(pr)) * (double)a.freq[pr]);
+            sh[tok * a.pairs + pr] = cs.x;
+            sh[(a.tb + tok) * a.pairs + pr] = cs.y;
         }
+        __syncthreads();
+        side_rows<T, V, UPL, BWD>(a, a.side[0], t0, nt, where[0][0], sh, sh + a.tb * a.pairs, w[0], acc[0]);
+        side_rows<T, V, UPL, BWD>(a, a.side[1], t0, nt, where[1][0], sh, sh + a.tb * a.pairs, w[1], acc[1]);
     }
     if (!BWD || a.part == nullptr) return;
     // sums of this workgroup: over the rows of a wave by exchanges, over the waves through LDS
@@ -238,8 +272,8 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a)
 #pragma unroll
         for (int i = 0; i < 2 * V; ++i)
             for (int o = a.lpr; o < 64; o <<= 1) {
-                sq[p][i] += __shfl_xor(sq[p][i], o);
-                sk[p][i] += __shfl_xor(sk[p][i], o);
+                acc[0][p][i] += __shfl_xor(acc[0][p][i], o);
+                acc[1][p][i] += __shfl_xor(acc[1][p][i], o);
             }
     for (int w = 0; w < 4; ++w) {
         if ((tid >> 6) == w && (tid & 63) < a.lpr) {
@@ -250,8 +284,8 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a)
                 for (int i = 0; i < 2 * V; ++i) {
                     const int e = (i < V ? t.o1 + i : t.o2 + i - V);
                     if (!t.on || (i >= V && !t.two)) continue;
-                    sh[e] = (w ? sh[e] : 0.f) + sq[p][i];
-                    sh[a.D + e] = (w ? sh[a.D + e] : 0.f) + sk[p][i];
+                    sh[e] = (w ? sh[e] : 0.f) + acc[0][p][i];
+                    sh[a.D + e] = (w ? sh[a.D + e] : 0.f) + acc[1][p][i];
                 }
             }
         }
@@ -260,18 +294,27 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a)
     for (int i = tid; i < 2 * a.D; i += 256) a.part[(size_t)blockIdx.x * 2 * a.D + i] = sh[i];
 }
 
-// dw: the workgroups' rows of 2 D sums.  A workgroup owns 16 columns, 16 threads walk the rows of each.
-__global__ __launch_bounds__(256) void weight_kernel(const float *__restrict__ part, int rows, int d, float *__restrict__ dqw, float *__restrict__ dkw)
+// dw: the workgroups' rows of 2 D sums.  A workgroup owns 16 columns, 64 threads walk the rows of each.
+__global__ __launch_bounds__(1024) void weight_kernel(const float *__restrict__ part, int rows, int d, float *__restrict__ dqw, float *__restrict__ dkw)
 {
-    __shared__ float red[16][17];
+    __shared__ float red[64][17];
     const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4, c = blockIdx.x * 16 + cx;
     float s = 0.f;
-    if (c < 2 * d)
-        for (int r = ry; r < rows; r += 16) s += part[(size_t)r * 2 * d + c];
+    if (c < 2 * d) {
+#pragma unroll 4
+        for (int r = ry; r < rows; r += 64) s += part[(size_t)r * 2 * d + c];
+    }
     red[ry][cx] = s;
     __syncthreads();
+    if (ry < 4) {
+        s = 0.f;
+        for (int r = 0; r < 16; ++r) s += red[ry * 16 + r][cx];
+    }
+    __syncthreads();
+    if (ry < 4) red[ry][cx] = s;
+    __syncthreads();
     if (ry == 0 && c < 2 * d) {
-        for (int r = 1; r < 16; ++r) s += red[r][cx];
+        s = (red[0][cx] + red[1][cx]) + (red[2][cx] + red[3][cx]);
         if (c < d) {
             if (dqw) dqw[c] = s;
         } else if (dkw) dkw[c - d] = s;
@@ -279,7 +322,7 @@ __global__ __launch_bounds__(256) void weight_kernel(const float *__restrict__ p
 }
 
 // widest piece that every row start and every piece of a row is a multiple of
-int piece(int dtype, int d, int pairs, int interleaved, long mask)
+int piece(int dtype, int d, int pairs, long mask)
 {
     const int most = dtype == F32 ? 4 : 8;
     const long es = dtype == F32 ? 4 : 2;
@@ -288,16 +331,21 @@ int piece(int dtype, int d, int pairs, int interleaved, long mask)
     return 1;
 }
 
-int groups_of(long tokens, int tb) { return (int)((tokens + tb - 1) / tb < 1024 ? (tokens + tb - 1) / tb : 1024); }
-
-// Tokens of a workgroup's turn: four rows per row slot, so that the angles are shared and loads overlap, while there are workgroups enough (four per
-// CU) -- else fewer, down to one token.
-int turn_tokens(long tokens, int heads, int lpr)
+// Tokens of a workgroup's turn: ten rows per row slot, so that the angles and the barriers are shared and loads overlap, while there are workgroups
+// enough (four per CU) -- else fewer, down to one token.  Backward: turns of one size that deal the tokens evenly to the resident workgroups.
+int turn_tokens(long tokens, int heads, int lpr, bool bwd)
 {
-    long tb = pa_div_up(4 * (256 / lpr), heads);
+    long tb = pa_div_up(10 * (256 / lpr), heads);
+    tb = tb > MAXTOK ? MAXTOK : tb;
+    if (bwd) {
+        const long each = (tokens + MAXGROUPS - 1) / MAXGROUPS, turns = (each + tb - 1) / tb;
+        return (int)((each + turns - 1) / turns);
+    }
     while (tb > 1 && tokens / tb < 1024) tb >>= 1;
-    return tb < 1 ? 1 : tb > MAXTOK ? MAXTOK : (int)tb;
+    return (int)tb;
 }
+
+int groups_of(long tokens, int tb) { return (int)((tokens + tb - 1) / tb < MAXGROUPS ? (tokens + tb - 1) / tb : MAXGROUPS); }
 
 template <typename T, bool BWD>
 void launch_norm(const NormArgs &a, int v, dim3 grid, size_t lds, hipStream_t st)
@@ -314,6 +362,7 @@ int norm_check(const char *name, int dtype, int b, int n, int h, int hk, int d, 
 {
     PA_REQUIRE(dtype >= F32 && dtype <= BF16, "%s: dtype %d is none of 0 (float32), 1 (float16), 2 (bfloat16)", name, dtype);
     PA_REQUIRE(b >= 0 && n >= 0 && h >= 0 && hk >= 0 && h + hk > 0 && h <= 65536 && hk <= 65536, "%s: bad sizes b=%d n=%d h=%d hk=%d", name, b, n, h, hk);
+    PA_REQUIRE((long)b * n <= (1l << 30), "%s: %ld tokens exceed 2^30", name, (long)b * n);
     PA_REQUIRE(d > 0 && d <= MAXD, "%s: head width %d is not in 1..%d", name, d, MAXD);
     PA_REQUIRE(axes >= 0 && per >= 0 && axes <= MAXD && per <= MAXD && 2 * axes * per <= d, "%s: %d axes of %d frequencies rotate more than %d elements", name, axes, per, d);
     PA_REQUIRE(axes * per == 0 || (pos && freq), "%s: null positions / frequencies", name);
@@ -323,15 +372,19 @@ int norm_check(const char *name, int dtype, int b, int n, int h, int hk, int d, 
 }
 
 // fills sizes, piece width and launch shape; returns the piece width
-int norm_plan(NormArgs &a, int dtype, int b, long mask)
+int norm_plan(NormArgs &a, int dtype, int b, bool bwd, long mask)
 {
     a.pairs = a.axes * a.per;
-    a.tokens = (long)b * a.N;
-    const int v = piece(dtype, a.D, a.pairs, a.interleaved, mask);
+    a.tokens = (int)((long)b * a.N);
+    a.dn = Div(a.N > 0 ? a.N : 1);
+    for (Side &s : a.side) s.d = Div(s.heads > 0 ? s.heads : 1);
+    a.dpairs = Div(a.pairs > 0 ? a.pairs : 1);
+    a.dper = Div(a.per > 0 ? a.per : 1);
+    const int v = piece(dtype, a.D, a.pairs, mask);
     a.units = pa_div_up(a.D, 2 * v);
     a.lpr = 1;
     while (a.lpr < a.units && a.lpr < 64) a.lpr <<= 1;
-    a.tb = turn_tokens(a.tokens, a.H + a.Hk, a.lpr);
+    a.tb = turn_tokens(a.tokens, a.side[0].heads + a.side[1].heads, a.lpr, bwd);
     return v;
 }
 
@@ -355,11 +408,12 @@ PA_API int pa_qk_norm_rotary(int dtype, int b, int n, int h, int hk, int d, cons
     if (b == 0 || n == 0) return PA_OK;
     PA_REQUIRE((h == 0 || (q && q_out)) && (hk == 0 || (k && k_out)), "pa_qk_norm_rotary: null tensor");
     NormArgs a = {};
-    a.q = q; a.k = k; a.oq = q_out; a.ok = k_out; a.qw = qw; a.kw = kw; a.pos = pos; a.freq = freq;
-    a.qb = qb; a.qn = qn; a.qh = qh; a.kb = kb; a.kn = kn; a.kh = kh; a.pb = pb;
-    a.N = n; a.H = h; a.Hk = hk; a.D = d; a.axes = axes; a.per = per; a.interleaved = interleaved; a.wtype = w_f32; a.ptype = ptype; a.eps = eps;
+    a.side[0] = {q, nullptr, qw, q_out, qb, qn, qh, 0, 0, 0, h, Div()};
+    a.side[1] = {k, nullptr, kw, k_out, kb, kn, kh, 0, 0, 0, hk, Div()};
+    a.pos = pos; a.freq = freq; a.pb = pb;
+    a.N = n; a.D = d; a.axes = axes; a.per = per; a.interleaved = interleaved; a.wtype = w_f32; a.ptype = ptype; a.eps = eps;
     const int es = dtype == F32 ? 4 : 2;
-    const int v = norm_plan(a, dtype, b, mask_of(es, {q, k, q_out, k_out}, {qb, qn, qh, kb, kn, kh, d}));
+    const int v = norm_plan(a, dtype, b, false, mask_of(es, {q, k, q_out, k_out}, {qb, qn, qh, kb, kn, kh, d}));
     const long groups = (a.tokens + a.tb - 1) / a.tb;
     PA_REQUIRE(groups < (1l << 31), "pa_qk_norm_rotary: too many workgroups");
     const size_t lds = (size_t)2 * a.tb * a.pairs * 4;
@@ -371,7 +425,7 @@ PA_API int pa_qk_norm_rotary(int dtype, int b, int n, int h, int hk, int d, cons
     return PA_OK;
 }
 
-PA_API long pa_qk_norm_rotary_backward_scratch_floats(int b, int n, int d) { return b <= 0 || n <= 0 || d <= 0 ? 0 : ((long)b * n < 1024 ? (long)b * n : 1024) * 2 * d; }
+PA_API long pa_qk_norm_rotary_backward_scratch_floats(int b, int n, int d) { return b <= 0 || n <= 0 || d <= 0 ? 0 : ((long)b * n < MAXGROUPS ? (long)b * n : MAXGROUPS) * 2 * d; }
 
 PA_API int pa_qk_norm_rotary_backward(int dtype, int b, int n, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn,
                                       long kh, const void *qw, const void *kw, int w_f32, const void *pos, int ptype, long pb, const float *freq, int axes,
@@ -383,12 +437,13 @@ PA_API int pa_qk_norm_rotary_backward(int dtype, int b, int n, int h, int hk, in
     if (b == 0 || n == 0) return PA_OK;
     PA_REQUIRE((h == 0 || (q && gq && dq)) && (hk == 0 || (k && gk && dk)) && (!(dqw || dkw) || scratch), "pa_qk_norm_rotary_backward: null tensor");
     NormArgs a = {};
-    a.q = q; a.k = k; a.gq = gq; a.gk = gk; a.oq = dq; a.ok = dk; a.qw = qw; a.kw = kw; a.pos = pos; a.freq = freq;
-    a.qb = qb; a.qn = qn; a.qh = qh; a.kb = kb; a.kn = kn; a.kh = kh; a.gqb = gqb; a.gqn = gqn; a.gqh = gqh; a.gkb = gkb; a.gkn = gkn; a.gkh = gkh; a.pb = pb;
-    a.N = n; a.H = h; a.Hk = hk; a.D = d; a.axes = axes; a.per = per; a.interleaved = interleaved; a.wtype = w_f32; a.ptype = ptype; a.eps = eps;
+    a.side[0] = {q, gq, qw, dq, qb, qn, qh, gqb, gqn, gqh, h, Div()};
+    a.side[1] = {k, gk, kw, dk, kb, kn, kh, gkb, gkn, gkh, hk, Div()};
+    a.pos = pos; a.freq = freq; a.pb = pb;
+    a.N = n; a.D = d; a.axes = axes; a.per = per; a.interleaved = interleaved; a.wtype = w_f32; a.ptype = ptype; a.eps = eps;
     a.part = dqw || dkw ? scratch : nullptr;
     const int es = dtype == F32 ? 4 : 2;
-    const int v = norm_plan(a, dtype, b, mask_of(es, {q, k, gq, gk, dq, dk}, {qb, qn, qh, kb, kn, kh, gqb, gqn, gqh, gkb, gkn, gkh, d}));
+    const int v = norm_plan(a, dtype, b, true, mask_of(es, {q, k, gq, gk, dq, dk}, {qb, qn, qh, kb, kn, kh, gqb, gqn, gqh, gkb, gkn, gkh, d}));
     const int groups = groups_of(a.tokens, a.tb);
     size_t lds = (size_t)2 * a.tb * a.pairs * 4;
     if (lds < (size_t)2 * d * 4) lds = (size_t)2 * d * 4;
@@ -396,7 +451,7 @@ PA_API int pa_qk_norm_rotary_backward(int dtype, int b, int n, int h, int hk, in
     if (dtype == F32) launch_norm<float, true>(a, v, dim3(groups), lds, st);
     else if (dtype == F16) launch_norm<_Float16, true>(a, v, dim3(groups), lds, st);
     else launch_norm<__bf16, true>(a, v, dim3(groups), lds, st);
-    if (a.part) hipLaunchKernelGGL(weight_kernel, dim3(pa_div_up(2 * d, 16)), dim3(256), 0, st, a.part, groups, d, dqw, dkw);
+    if (a.part) hipLaunchKernelGGL(weight_kernel, dim3(pa_div_up(2 * d, 16)), dim3(1024), 0, st, a.part, groups, d, dqw, dkw);
     PA_CHECK_LAUNCH("pa_qk_norm_rotary_backward");
     return PA_OK;
 }
