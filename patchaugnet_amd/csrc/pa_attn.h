@@ -37,6 +37,10 @@ __device__ __forceinline__ long xcd_item(long x, long n)
     return k * each + (k < rest ? k : rest) + (x >> 3);
 }
 
+template <int X> struct Const {
+    __device__ constexpr int operator()() const { return X; }
+};
+
 template <typename T> struct Frag;
 template <> struct Frag<float> { typedef pa_f8 type; };
 template <> struct Frag<_Float16> { typedef pa_h8 type; };
@@ -130,18 +134,18 @@ __device__ __forceinline__ pa_u4 ldg16(const void *p, bool ok)
 // elements from d on arrive as zeros, whatever is in memory there (checked only for tiles and widths that have any).
 template <typename T, int DT, int R, int NT> struct Stage {
     typedef Tile<T, DT> L;
-    static constexpr int N = R * L::CH / NT;
-    static_assert(R * L::CH % NT == 0, "a tile splits evenly over the workgroup");
+    static constexpr int ALL = R * L::CH, N = (ALL + NT - 1) / NT;
     u32 off[N];
     pa_u4 x[N];
 
+    __device__ static __forceinline__ bool mine(int u) { return ALL % NT == 0 || (int)(threadIdx.x + u * NT) < ALL; }
     __device__ static __forceinline__ int row(int u) { return (int)(threadIdx.x + u * NT) / L::CH; }
     __device__ static __forceinline__ int chunk(int u) { return (int)(threadIdx.x + u * NT) - row(u) * L::CH; }
     // rows `stride` elements apart
     __device__ __forceinline__ void strided(long stride)
     {
 #pragma unroll
-        for (int u = 0; u < N; ++u) off[u] = ((u32)row(u) * (u32)stride + chunk(u) * L::EC) * (u32)sizeof(T);
+        for (int u = 0; u < N; ++u) off[u] = mine(u) ? ((u32)row(u) * (u32)stride + chunk(u) * L::EC) * (u32)sizeof(T) : 0u;
     }
     __device__ __forceinline__ void fetch(const T *base, int valid, int d)
     {
@@ -162,7 +166,8 @@ template <typename T, int DT, int R, int NT> struct Stage {
     __device__ __forceinline__ void store(char *s) const
     {
 #pragma unroll
-        for (int u = 0; u < N; ++u) *reinterpret_cast<pa_u4 *>(s + L::at(row(u), chunk(u))) = x[u];
+        for (int u = 0; u < N; ++u)
+            if (mine(u)) *reinterpret_cast<pa_u4 *>(s + L::at(row(u), chunk(u))) = x[u];
     }
 };
 

@@ -78,14 +78,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(co
     float m_run = -INFINITY, l_run = 0.f;
 
     if (t0 < t1) fetch(tiles.tile(t0));
-    for (int it = t0; it < t1; ++it) {
-        char *ks = smem + ((it - t0) & 1) * 2 * TB, *vs = ks + TB;
+    auto step = [&](int it, auto half) {
+        char *ks = smem + half() * 2 * TB, *vs = ks + TB;
         sk.store(ks);
         sv.store(vs);
         __syncthreads();                                       // the previous tile's readers of this half passed the barrier before this one
         const int j0 = tiles.tile(it) * KT;
         if (it + 1 < t1) fetch(tiles.tile(it + 1));
-        if (!wave_on) continue;
+        if (!wave_on) return;
 #pragma unroll
         for (int sub = 0; sub < KT / 32; ++sub) {
             const int js = j0 + sub * 32;
@@ -123,6 +123,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(co
                 for (int ct = 0; ct < DT / 32; ++ct) mma(o[ct], L::ldt(vs, sub * 32 + 16 * u, ct * 32), p);
             }
         }
+    };
+    for (int it = t0; it < t1; it += 2) {                      // two halves of LDS, two copies of the step: places in LDS are constants
+        step(it, Const<0>());
+        if (it + 1 < t1) step(it + 1, Const<1>());
     }
 
     l_run += other_half(l_run);
