@@ -259,9 +259,14 @@ template <int KT> struct TileList {
     __device__ __forceinline__ int tile(int i) const { return i < nsk ? i : lo + i - nsk; }
 };
 
-// Waves of a workgroup, each with 32 rows (or keys): four share a tile's way into LDS; two make the grid finer, which counts while there are few
-// rounds of workgroups, since the last round is seldom full.  `four`: workgroups of four waves that the problem makes.
-static inline int waves_of(long four) { return four < 2048 ? 2 : 4; }
+// Waves of a workgroup, each with 32 rows (or keys).  Four share a tile's way into LDS; with two, the keys that a workgroup walks reach less beyond its
+// own rows and float32 needs fewer registers for tiles on their way.  Measured, us with four / two waves: forward bf16 4 x 4096 x 16 heads of 64, window
+// 512: 62 / 83; 16384 tokens of 128, window 1024: 748 / 832; float32 4 x 2048 x 8 of 64 and 128, window 256: 64 / 60 and 142 / 127; dk and dv of the
+// latter 209 / 184 and 454 / 447, of fp16 8 x 4096 x 8 of 96 with 64 keys either side 122 / 103, of bf16 4 x 2048 x 16 of 64, all keys: 193 / 236.
+static inline int waves_of(int es, long reach) { return es == 4 || reach < 256 ? 2 : 4; }
+
+// waves on a SIMD that the registers are held down to
+template <typename T, int DT> constexpr int waves_per_simd() { return sizeof(T) == 2 ? 2 : DT <= 32 ? 3 : DT <= 64 ? 2 : 1; }
 
 // Keys of a tile of the kernels that own rows: fewer where two waves alone bring wide rows into LDS (registers).
 template <typename T, int DT, int NW> constexpr int key_tile() { return NW == 2 && DT * (int)sizeof(T) >= 256 ? 32 : 64; }

@@ -209,9 +209,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a)
     const int runs = (tiles.n + a.tpc - 1) / a.tpc;
     const float *pm = a.part + (size_t)a.runs * all * DT;
     float m = -INFINITY, l = 0.f;
+#pragma unroll 8
     for (int s = 0; s < runs; ++s) m = fmaxf(m, pm[(s * all + at) * 2]);
     const float mref = m > -INFINITY ? m : 0.f;
     pa_f4 o = (pa_f4)(0.f);
+#pragma unroll 8
     for (int s = 0; s < runs; ++s) {
         const float w = ex2(pm[(s * all + at) * 2] - mref);
         l += w * pm[(s * all + at) * 2 + 1];

@@ -2,7 +2,7 @@
 //
 //     o_i = sum_j P_ij v_j,   P_ij = exp(s_ij) / sum_j exp(s_ij),   s_ij = scale q_i . k_j   over the keys j in view of row i (View, pa_attn.h)
 //
-// One pass over the keys with a running maximum and sum: O(window) work and nothing N x M in memory.  A workgroup owns 128 (64) rows -- the N queries of
+// One pass over the keys with a running maximum and sum: O(window) work and nothing N x M in memory.  A workgroup owns 128 (float32: 64) rows -- the N queries of
 // the G heads that share a key head, query-major, so that one tile of keys serves all of them -- and walks the 64-key tiles that its rows can see:
 // the tiles of the first tokens, then one contiguous range.  A wave owns 32 rows.  S^T = K Q^T puts one row into a lane's registers (maximum and
 // sum need one exchange between the two half waves), and the registers of P^T feed O^T += V^T P^T without leaving the lane; V is read transposed
@@ -28,7 +28,7 @@ struct FwdArgs {
 };
 
 template <typename T, int DT, int NW, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void fwd_kernel(const FwdArgs a)
+__global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel(const FwdArgs a)
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
@@ -169,9 +169,11 @@ __global__ __launch_bounds__(256) void join_kernel(const FwdArgs a)
     if (at >= all) return;
     const float *pm = a.part + (size_t)a.splits * all * DT;
     float m = -INFINITY, l = 0.f;
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) m = fmaxf(m, pm[(s * all + at) * 2]);
     const float mref = m > -INFINITY ? m : 0.f;
     pa_f4 o = (pa_f4)(0.f);
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) {
         const float w = ex2(pm[(s * all + at) * 2] - mref);
         l += w * pm[(s * all + at) * 2 + 1];
@@ -190,11 +192,11 @@ struct Shape {
 
 // Work is split over the keys when the rows alone leave the chip idle: fewer than 256 workgroups (one per CU).  Two per CU are aimed at, each with
 // at least four tiles, because a part costs one round trip of its rows in 32 bits.
-Shape shape_of(int B, int N, int M, int H, int Hk, int left, int right, int sinks)
+Shape shape_of(int B, int N, int M, int H, int Hk, int es, int left, int right, int sinks)
 {
     const long G = H / Hk, rows = (long)N * G;
     Shape s;
-    s.waves = waves_of((long)B * Hk * ((rows + 127) / 128));
+    s.waves = waves_of(es, UNBOUNDED);
     s.nqt = pa_div_up(rows, 32 * s.waves);
     s.splits = 1;
     const long wgs = (long)B * Hk * s.nqt;
@@ -216,16 +218,15 @@ void launch_rows(const FwdArgs &a, hipStream_t st)
 }
 
 template <typename T, int DT>
-int launch_fwd(const FwdArgs &a, int waves, hipStream_t st)
+int launch_fwd(const FwdArgs &a, hipStream_t st)
 {
-    if (a.splits > 1) {                                        // few rows: always two waves
-        launch_rows<T, DT, 2, true>(a, st);
+    constexpr int NW = sizeof(T) == 4 ? 2 : 4;
+    if (a.splits > 1) {
+        launch_rows<T, DT, NW, true>(a, st);
         const long threads = (long)a.B * a.Hk * a.N * a.G * (DT / 4);
         hipLaunchKernelGGL((join_kernel<T, DT>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
-    } else if (waves == 2) {
-        launch_rows<T, DT, 2, false>(a, st);
     } else {
-        launch_rows<T, DT, 4, false>(a, st);
+        launch_rows<T, DT, NW, false>(a, st);
     }
     return 0;
 }
@@ -236,7 +237,7 @@ PA_API long pa_window_attention_scratch_floats(int b, int n, int m, int h, int h
 {
     if (b <= 0 || n <= 0 || h <= 0 || hk <= 0 || h % hk != 0) return 0;
     const int l = left < 0 ? UNBOUNDED : left, r = right < 0 ? UNBOUNDED : right;
-    const int s = shape_of(b, n, m, h, hk, l, r, sinks).splits;
+    const int s2 = shape_of(b, n, m, h, hk, 2, l, r, sinks).splits, s4 = shape_of(b, n, m, h, hk, 4, l, r, sinks).splits, s = s2 > s4 ? s2 : s4;
     return s <= 1 ? 0 : (long)s * b * n * h * (width(d) + 2);
 }
 
@@ -256,14 +257,14 @@ PA_API int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, in
     a.view.start = start; a.view.length = length;
     a.c = scale * 1.4426950408889634f;
     a.g = Div(a.G);
-    const Shape sh = shape_of(b, n, m, h, hk, a.view.left, a.view.right, sinks);
+    const Shape sh = shape_of(b, n, m, h, hk, dtype == PA_DT_F32 ? 4 : 2, a.view.left, a.view.right, sinks);
     a.nqt = sh.nqt;
     a.splits = sh.splits;
     PA_REQUIRE(kn >= 0 && vn >= 0 && kn <= PA_ATTN_MAXSTRIDE && vn <= PA_ATTN_MAXSTRIDE, "pa_window_attention: tokens are more than 2^22 elements apart");
     PA_REQUIRE((long)a.nqt * b * hk < (1l << 31), "pa_window_attention: too many workgroups");
     PA_REQUIRE(a.splits == 1 || scratch, "pa_window_attention: this size needs pa_window_attention_scratch_floats() of scratch");
     hipStream_t st = (hipStream_t)stream;
-#define FWD(T, DT) launch_fwd<T, DT>(a, sh.waves, st)
+#define FWD(T, DT) launch_fwd<T, DT>(a, st)
     PA_ATTN_DISPATCH(dtype, d, FWD);
 #undef FWD
     PA_CHECK_LAUNCH("pa_window_attention");

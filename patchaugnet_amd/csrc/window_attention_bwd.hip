@@ -39,7 +39,7 @@ struct BwdArgs {
 };
 
 template <typename T, int DT, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void dq_kernel(const BwdArgs a)
+__global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(const BwdArgs a)
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
@@ -137,7 +137,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void dq_kernel(con
         }
 }
 
-// What a workgroup of the dk, dv launch owns: a slice of the far rows of 32 first tokens (these come first), or a slice of a key tile's window.
+// What a workgroup of the dk, dv launch owns: a slice of a key tile's window, or (behind them in the launch: they are short and fill its last round) a
+// slice of the far rows of 32 first tokens.
 struct Walk {
     int bh, k0, slice, slices;          // keys from k0
     bool far;
@@ -145,9 +146,10 @@ struct Walk {
 
     __device__ __forceinline__ Walk(const BwdArgs &a, long id, int kb, int nw)
     {
-        const long nfar = (long)a.B * a.Hk * a.groups * a.fars;
-        far = id < nfar;
+        const long nwin = (long)a.B * a.Hk * a.nkt * a.slices, nfar = (long)a.B * a.Hk * a.groups * a.fars;
+        far = id >= nwin;
         if (far) {
+            id -= nwin;
             slot = id * 32 * nw;
             slices = a.fars;
             slice = (int)(id % slices);
@@ -155,7 +157,7 @@ struct Walk {
             k0 = (int)(id % a.groups) * 32;
             bh = (int)(id / a.groups);
         } else {
-            id -= nfar;
+            id = xcd_item(id, nwin);
             const long at = id;
             slices = a.slices;
             slice = (int)(id % slices);
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
     constexpr int KB = 32 * NW, RT = row_tile<T, DT>(), TB = RT * L::RB, BUF = 2 * TB + 3 * RT * 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][Q tile, dO tile, lse, delta, position]
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
-    const Walk w(a, xcd_item(blockIdx.x, gridDim.x), KB, NW);
+    const Walk w(a, blockIdx.x, KB, NW);
     const int b = w.bh / a.Hk, hk = w.bh - b * a.Hk;
     const int len = a.view.len(b), start = a.view.first(b);
 
@@ -303,6 +305,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
             }
         }
     }
+    if (w.far && j >= a.view.sinks) return;                     // nobody reads those
     if (w.slot >= 0) {
         float *po = a.part + ((size_t)w.slot + wave * 32 + (l & 31)) * (2 * DT);
 #pragma unroll
@@ -331,27 +334,33 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
         }
 }
 
-// dk, dv of the key tiles that left partial sums: the window's slices in their order, then the far rows' (slice by slice, wave by wave).  A thread owns
-// four elements of dk or dv of a key.
+// dk, dv of the key tiles that left partial sums: the window's slices, then the far rows' (slice by slice, wave by wave).  A workgroup owns a key;
+// DT / 2 threads hold a row of dk and dv, four elements each, the 512 / DT groups of such threads take the sums in turn and are added in order.
 template <typename T, int DT, int NW>
 __global__ __launch_bounds__(256) void dkv_join_kernel(const BwdArgs a, int tiles)
 {
-    constexpr int C = DT / 2, KB = 32 * NW;
-    const long id = ((long)blockIdx.x * 256 + threadIdx.x) / C;
-    const int c = (int)(((long)blockIdx.x * 256 + threadIdx.x) % C) * 4;
-    const long tile = id / KB;
-    const int r = (int)(id % KB);
-    if (tile >= (long)a.B * a.Hk * tiles) return;
+    constexpr int C = DT / 2, P = 256 / C, KB = 32 * NW;
+    __shared__ pa_f4 red[P][C];
+    const int c = (int)threadIdx.x % C * 4, part = (int)threadIdx.x / C;
+    const long tile = blockIdx.x / KB;
+    const int r = (int)(blockIdx.x % KB);
     const int bh = (int)(tile / tiles), t = (int)(tile % tiles), b = bh / a.Hk, hk = bh - b * a.Hk, j = t * KB + r;
     if (j >= a.view.m) return;
     const size_t nfar = (size_t)a.B * a.Hk * a.groups * a.fars * 32 * NW;
     const float *p = a.part + (nfar + (size_t)tile * a.slices * KB + r) * (2 * DT) + c;
     pa_f4 s = (pa_f4)(0.f);
-    for (int i = 0; i < a.slices; ++i) s += *reinterpret_cast<const pa_f4 *>(p + (size_t)i * KB * 2 * DT);
-    if (j / 32 < a.groups) {
+#pragma unroll 4
+    for (int i = part; i < a.slices; i += P) s += *reinterpret_cast<const pa_f4 *>(p + (size_t)i * KB * 2 * DT);
+    if (j < a.view.sinks && a.groups > 0) {
         p = a.part + (((size_t)bh * a.groups + j / 32) * a.fars * 32 * NW + (j & 31)) * (2 * DT) + c;
-        for (int i = 0; i < a.fars * NW; ++i) s += *reinterpret_cast<const pa_f4 *>(p + (size_t)i * 32 * 2 * DT);
+#pragma unroll 8
+        for (int i = part; i < a.fars * NW; i += P) s += *reinterpret_cast<const pa_f4 *>(p + (size_t)i * 32 * 2 * DT);
     }
+    if (part < P) red[part][c / 4] = s;
+    __syncthreads();
+    if (part > 0) return;
+#pragma unroll
+    for (int i = 1; i < P; ++i) s += red[i][c / 4];
     const size_t at = (((size_t)b * a.view.m + j) * a.Hk + hk) * a.D;
     if (c < DT) {
         if (c < a.D) st4<T>((T *)a.dk + at + c, s[0] * a.scale, s[1] * a.scale, s[2] * a.scale, s[3] * a.scale);
@@ -369,15 +378,16 @@ struct Shape {
     int joined() const { return slices > 1 ? nkt : groups > 0 ? nst : 0; }      // key tiles with partial sums
 };
 
-// Slices: keys that do not fill the chip (fewer than 2048 waves, two per SIMD) have their walks cut, each slice with at least four row tiles; far rows into slices of
-// twice as many row tiles, on each of which one wave works.
+// Slices: keys that do not fill the chip (fewer than 2048 waves, two per SIMD) have their walks cut, each slice with at least four row tiles;
+// far rows are cut into slices of
+// 16 row tiles.
 Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int right, int sinks, bool started)
 {
     Shape s;
     const long G = H / Hk, bh = (long)B * Hk, rows = (long)N * G;
-    s.qwaves = waves_of(bh * ((rows + 127) / 128));
+    s.qwaves = waves_of(es, UNBOUNDED);
     s.nqt = pa_div_up(rows, 32 * s.qwaves);
-    s.kwaves = waves_of(bh * ((M + 127l) / 128));
+    s.kwaves = waves_of(es, (long)left + right);
     const int kb = 32 * s.kwaves, rt = width(d) * es >= 512 ? 32 : 64;
     s.rt = G <= rt ? rt / (int)G * (int)G : rt;
     s.nkt = pa_div_up(M, kb);
@@ -389,9 +399,8 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int 
     const bool far = first > 0 && (started ? left < M : left < N - 1);          // rows behind the window of the first tokens
     s.groups = far ? pa_div_up(first, 32) : 0;
     s.nst = pa_div_up(first, kb);
-    const long per = (walk + s.slices - 1) / s.slices;                          // row tiles of a slice
-    const long f = pa_div_up(rows, s.rt) / (2 * per > 8 ? 2 * per : 8) + 1;
-    s.fars = far ? (f > 64 ? 64 : (int)f) : 1;
+    const long f = (rows + 16 * s.rt - 1) / (16 * s.rt);
+    s.fars = far ? (f > 64 ? 64 : f < 1 ? 1 : (int)f) : 1;
     return s;
 }
 
@@ -410,18 +419,16 @@ void launch_dkv(const BwdArgs &a, int joined, hipStream_t st)
     if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&dkv_kernel<T, DT, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     const long bh = (long)a.B * a.Hk;
     hipLaunchKernelGGL((dkv_kernel<T, DT, NW>), dim3((unsigned)(bh * a.groups * a.fars + bh * a.nkt * a.slices)), dim3(64 * NW), lds, st, a);
-    if (joined) hipLaunchKernelGGL((dkv_join_kernel<T, DT, NW>), dim3((unsigned)(bh * joined * 32 * NW * (DT / 2) / 256)), dim3(256), 0, st, a, joined);
+    if (joined) hipLaunchKernelGGL((dkv_join_kernel<T, DT, NW>), dim3((unsigned)(bh * joined * 32 * NW)), dim3(256), 0, st, a, joined);
 }
 
 template <typename T, int DT>
 int launch_bwd(const BwdArgs &a, const Shape &s, hipStream_t st)
 {
-    if (a.nqt) {
-        if (s.qwaves == 2) launch_dq<T, DT, 2>(a, st);
-        else launch_dq<T, DT, 4>(a, st);
-    }
+    if (a.nqt) launch_dq<T, DT, sizeof(T) == 4 ? 2 : 4>(a, st);
     if (a.nkt) {
-        if (s.kwaves == 2) launch_dkv<T, DT, 2>(a, s.joined(), st);
+        if constexpr (sizeof(T) == 4) launch_dkv<T, DT, 2>(a, s.joined(), st);
+        else if (s.kwaves == 2) launch_dkv<T, DT, 2>(a, s.joined(), st);
         else launch_dkv<T, DT, 4>(a, s.joined(), st);
     }
     return 0;
