@@ -129,6 +129,14 @@ __device__ __forceinline__ pa_u4 ldg16(const void *p, bool ok)
     return z;
 }
 
+// A per-thread offset, fixed for the whole kernel, at the place of its use.  Without this the compiler (ROCm 7.2) keeps the 64-bit form of the offset
+// across the loop and, where one way of a fetch is masked, computes it in some lanes only: the other lanes then load from anywhere.
+__device__ __forceinline__ u32 here(u32 x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // R rows of a tensor on their way into an LDS tile: NT threads, 16-byte chunks, fetched into registers and stored later.  A thread's places in a tile
 // are the same for every tile, so a fetch is one load per chunk at (uniform base of the tile) + (32-bit offset of the thread); rows from `valid` on and
 // elements from d on arrive as zeros, whatever is in memory there (checked only for tiles and widths that have any).
@@ -152,12 +160,13 @@ template <typename T, int DT, int R, int NT> struct Stage {
         const char *p = reinterpret_cast<const char *>(base);
         if (valid >= R && d == DT) {
 #pragma unroll
-            for (int u = 0; u < N; ++u) x[u] = *reinterpret_cast<const pa_u4 *>(p + off[u]);
+            for (int u = 0; u < N; ++u) x[u] = *reinterpret_cast<const pa_u4 *>(p + here(off[u]));
         } else {
 #pragma unroll
             for (int u = 0; u < N; ++u) {                       // row 0, chunk 0 is always there (valid >= 1): no branch around the load
                 const bool ok = row(u) < valid && chunk(u) * L::EC < d;
-                const pa_u4 t = *reinterpret_cast<const pa_u4 *>(p + (ok ? off[u] : 0u));
+                const u32 o = here(off[u]);
+                const pa_u4 t = *reinterpret_cast<const pa_u4 *>(p + (ok ? o : 0u));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[u][i] = ok ? t[i] : 0u;
             }
@@ -170,6 +179,47 @@ template <typename T, int DT, int R, int NT> struct Stage {
             if (mine(u)) *reinterpret_cast<pa_u4 *>(s + L::at(row(u), chunk(u))) = x[u];
     }
 };
+
+__device__ const pa_u4 pa_zeros = {0, 0, 0, 0};
+
+// R rows of a tensor straight from memory into an LDS tile (global_load_lds, 16 bytes a lane): no registers on the way.  A wave's lanes fill 64
+// neighbouring places, so the swizzle is in which chunk a lane asks for; rows from `valid` on and elements from d on are asked of a block of zeros.
+// The data is there for all waves after arrived() and a barrier.
+template <typename T, int DT, int R, int NT> struct Direct {
+    typedef Tile<T, DT> L;
+    static constexpr int ALL = R * L::CH, N = (ALL + NT - 1) / NT;
+    u32 off[N];
+
+    __device__ static __forceinline__ int row(int u) { return (int)(threadIdx.x + u * NT) / L::CH; }
+    __device__ static __forceinline__ int chunk(int u) { return ((int)(threadIdx.x + u * NT) - row(u) * L::CH) ^ L::swz(row(u)); }
+    __device__ __forceinline__ void strided(long stride)
+    {
+#pragma unroll
+        for (int u = 0; u < N; ++u) off[u] = ((u32)row(u) * (u32)stride + chunk(u) * L::EC) * (u32)sizeof(T);
+    }
+    __device__ __forceinline__ void fetch(char *tile, const T *base, int valid, int d) const
+    {
+        typedef const __attribute__((address_space(1))) void *gp;
+        typedef __attribute__((address_space(3))) void *lp;
+        const char *p = reinterpret_cast<const char *>(base);
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        if (valid >= R && d == DT) {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (ALL % NT == 0 || wave * 64 + u * NT < ALL) __builtin_amdgcn_global_load_lds((gp)(p + here(off[u])), (lp)(tile + (u * NT + wave * 64) * 16), 16, 0, 0);
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (ALL % NT == 0 || wave * 64 + u * NT < ALL) {
+                    const bool ok = row(u) < valid && chunk(u) * L::EC < d;
+                    const u32 o = here(off[u]);
+                    const char *g = ok ? p + o : reinterpret_cast<const char *>(&pa_zeros);
+                    __builtin_amdgcn_global_load_lds((gp)g, (lp)(tile + (u * NT + wave * 64) * 16), 16, 0, 0);
+                }
+        }
+    }
+};
+__device__ __forceinline__ void arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0): this wave's loads into LDS
 
 // eight accumulator registers as an operand fragment (one rounding to the operand type)
 template <typename T> __device__ __forceinline__ typename Frag<T>::type pack(const pa_f16v &a, int u)

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
     constexpr int KT = key_tile<T, DT, NW>(), TB = KT * L::RB, QT = 32 * NW;
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K tile, V tile]
+    __shared__ __attribute__((aligned(16))) char k0[TB], k1[TB], v0[TB], v1[TB];       // apart, so that loads into one hold up no reads of another
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
 
     const int item = (int)xcd_item(blockIdx.x, gridDim.x);
@@ -64,12 +64,12 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
     const int flo = max(wp1 - a.view.left, 0), fhi = min(wp0 + a.view.right, len - 1);                  // every row sees [flo, fhi]
 
     const T *kp = (const T *)a.k + b * a.kb + hk * a.kh, *vp = (const T *)a.v + b * a.vb + hk * a.vh;
-    Stage<T, DT, KT, 64 * NW> sk, sv;
+    Direct<T, DT, KT, 64 * NW> sk, sv;
     sk.strided(a.kn);
     sv.strided(a.vn);
-    auto fetch = [&](int t) {                                  // rows behind the sequence are zeros: what they hold never meets a product
-        sk.fetch(kp + (long)t * KT * a.kn, len - t * KT, a.D);
-        sv.fetch(vp + (long)t * KT * a.vn, len - t * KT, a.D);
+    auto fetch = [&](int t, char *ks, char *vs) {              // rows behind the sequence are zeros: what they hold never meets a product
+        sk.fetch(ks, kp + (long)t * KT * a.kn, len - t * KT, a.D);
+        sv.fetch(vs, vp + (long)t * KT * a.vn, len - t * KT, a.D);
     };
 
     pa_f16v o[DT / 32];
@@ -77,14 +77,12 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
     for (int ct = 0; ct < DT / 32; ++ct) o[ct] = (pa_f16v)(0.f);
     float m_run = -INFINITY, l_run = 0.f;
 
-    if (t0 < t1) fetch(tiles.tile(t0));
-    auto step = [&](int it, auto half) {
-        char *ks = smem + half() * 2 * TB, *vs = ks + TB;
-        sk.store(ks);
-        sv.store(vs);
-        __syncthreads();                                       // the previous tile's readers of this half passed the barrier before this one
+    if (t0 < t1) fetch(tiles.tile(t0), k0, v0);
+    auto step = [&](int it, char *ks, char *vs, char *kn, char *vn) {
+        arrived();
+        __syncthreads();                                       // the tile is there, and everyone is done with the one before it
         const int j0 = tiles.tile(it) * KT;
-        if (it + 1 < t1) fetch(tiles.tile(it + 1));
+        if (it + 1 < t1) fetch(tiles.tile(it + 1), kn, vn);
         if (!wave_on) return;
 #pragma unroll
         for (int sub = 0; sub < KT / 32; ++sub) {
@@ -125,8 +123,8 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
         }
     };
     for (int it = t0; it < t1; it += 2) {                      // two halves of LDS, two copies of the step: places in LDS are constants
-        step(it, Const<0>());
-        if (it + 1 < t1) step(it + 1, Const<1>());
+        step(it, k0, v0, k1, v1);
+        if (it + 1 < t1) step(it + 1, k1, v1, k0, v0);
     }
 
     l_run += other_half(l_run);
@@ -212,9 +210,7 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int es, int left, int right, 
 template <typename T, int DT, int NW, bool SPLIT>
 void launch_rows(const FwdArgs &a, hipStream_t st)
 {
-    constexpr int lds = 4 * key_tile<T, DT, NW>() * DT * (int)sizeof(T);
-    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&fwd_kernel<T, DT, NW, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    hipLaunchKernelGGL((fwd_kernel<T, DT, NW, SPLIT>), dim3((unsigned)((long)a.nqt * a.B * a.Hk), (unsigned)a.splits), dim3(64 * NW), lds, st, a);
+    hipLaunchKernelGGL((fwd_kernel<T, DT, NW, SPLIT>), dim3((unsigned)((long)a.nqt * a.B * a.Hk), (unsigned)a.splits), dim3(64 * NW), 0, st, a);
 }
 
 template <typename T, int DT>
