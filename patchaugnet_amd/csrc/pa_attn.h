@@ -137,53 +137,10 @@ __device__ __forceinline__ u32 here(u32 x)
     return x;
 }
 
-// R rows of a tensor on their way into an LDS tile: NT threads, 16-byte chunks, fetched into registers and stored later.  A thread's places in a tile
-// are the same for every tile, so a fetch is one load per chunk at (uniform base of the tile) + (32-bit offset of the thread); rows from `valid` on and
-// elements from d on arrive as zeros, whatever is in memory there (checked only for tiles and widths that have any).
-template <typename T, int DT, int R, int NT> struct Stage {
-    typedef Tile<T, DT> L;
-    static constexpr int ALL = R * L::CH, N = (ALL + NT - 1) / NT;
-    u32 off[N];
-    pa_u4 x[N];
-
-    __device__ static __forceinline__ bool mine(int u) { return ALL % NT == 0 || (int)(threadIdx.x + u * NT) < ALL; }
-    __device__ static __forceinline__ int row(int u) { return (int)(threadIdx.x + u * NT) / L::CH; }
-    __device__ static __forceinline__ int chunk(int u) { return (int)(threadIdx.x + u * NT) - row(u) * L::CH; }
-    // rows `stride` elements apart
-    __device__ __forceinline__ void strided(long stride)
-    {
-#pragma unroll
-        for (int u = 0; u < N; ++u) off[u] = mine(u) ? ((u32)row(u) * (u32)stride + chunk(u) * L::EC) * (u32)sizeof(T) : 0u;
-    }
-    __device__ __forceinline__ void fetch(const T *base, int valid, int d)
-    {
-        const char *p = reinterpret_cast<const char *>(base);
-        if (valid >= R && d == DT) {
-#pragma unroll
-            for (int u = 0; u < N; ++u) x[u] = *reinterpret_cast<const pa_u4 *>(p + here(off[u]));
-        } else {
-#pragma unroll
-            for (int u = 0; u < N; ++u) {                       // row 0, chunk 0 is always there (valid >= 1): no branch around the load
-                const bool ok = row(u) < valid && chunk(u) * L::EC < d;
-                const u32 o = here(off[u]);
-                const pa_u4 t = *reinterpret_cast<const pa_u4 *>(p + (ok ? o : 0u));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[u][i] = ok ? t[i] : 0u;
-            }
-        }
-    }
-    __device__ __forceinline__ void store(char *s) const
-    {
-#pragma unroll
-        for (int u = 0; u < N; ++u)
-            if (mine(u)) *reinterpret_cast<pa_u4 *>(s + L::at(row(u), chunk(u))) = x[u];
-    }
-};
-
 __device__ const pa_u4 pa_zeros = {0, 0, 0, 0};
 
-// R rows of a tensor straight from memory into an LDS tile (global_load_lds, 16 bytes a lane): no registers on the way.  A wave's lanes fill 64
-// neighbouring places, so the swizzle is in which chunk a lane asks for; rows from `valid` on and elements from d on are asked of a block of zeros.
+// R rows of a tensor straight from memory into an LDS tile by NT threads (global_load_lds, 16 bytes a lane): no registers on the way, one load per chunk
+// at (uniform base of the tile) + (32-bit offset of the thread, the same for every tile).  A wave's lanes fill 64 neighbouring places, so the swizzle is in which chunk a lane asks for; rows from `valid` on and elements from d on are asked of a block of zeros.
 // The data is there for all waves after arrived() and a barrier.
 template <typename T, int DT, int R, int NT> struct Direct {
     typedef Tile<T, DT> L;

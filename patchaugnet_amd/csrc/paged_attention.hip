@@ -37,7 +37,7 @@ __device__ __forceinline__ View view_of(const PagedArgs &a)
 }
 
 template <typename T, int DT>
-__global__ __launch_bounds__(256) void paged_kernel(const PagedArgs a)
+__global__ __launch_bounds__(256, (waves_per_simd<T, DT>())) void paged_kernel(const PagedArgs a)
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void paged_kernel(const PagedArgs a)
     F kf[NK];
     pa_u4 pv[NK * NP];
     u32 mask = 0;
-    auto fetch = [&](int t) {
+    auto fetch = [&](int t) __attribute__((always_inline)) {
         const int j = tiles.tile(t) * KT + (l & 31);
         bool ok = j < len && (j >= lo || j < a.sinks);
         int page = 0, at = 0;
@@ -76,6 +76,15 @@ __global__ __launch_bounds__(256) void paged_kernel(const PagedArgs a)
         }
         mask = (u32)__ballot(ok);
         const T *kr = kbase + (long)page * a.kp + (long)at * a.kt, *vr = vbase + (long)page * a.vp + (long)at * a.vt;
+        if (mask == 0xffffffffu && a.D == DT) {                 // the rule: no lane leaves anything out
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) kf[kk] = ldrow<T>(kr, kk, h, DT, true);
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int u = 0; u < NP; ++u) pv[kk * NP + u] = *reinterpret_cast<const pa_u4 *>(vr + 16 * kk + 8 * h + u * L::EC);
+            return;
+        }
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) kf[kk] = ldrow<T>(kr, kk, h, a.D, ok);
 #pragma unroll

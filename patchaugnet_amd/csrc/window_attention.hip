@@ -67,7 +67,7 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
     Direct<T, DT, KT, 64 * NW> sk, sv;
     sk.strided(a.kn);
     sv.strided(a.vn);
-    auto fetch = [&](int t, char *ks, char *vs) {              // rows behind the sequence are zeros: what they hold never meets a product
+    auto fetch = [&](int t, char *ks, char *vs) __attribute__((always_inline)) {              // rows behind the sequence are zeros: what they hold never meets a product
         sk.fetch(ks, kp + (long)t * KT * a.kn, len - t * KT, a.D);
         sv.fetch(vs, vp + (long)t * KT * a.vn, len - t * KT, a.D);
     };
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
     float m_run = -INFINITY, l_run = 0.f;
 
     if (t0 < t1) fetch(tiles.tile(t0), k0, v0);
-    auto step = [&](int it, char *ks, char *vs, char *kn, char *vn) {
+    auto step = [&](int it, char *ks, char *vs, char *kn, char *vn) __attribute__((always_inline)) {
         arrived();
         __syncthreads();                                       // the tile is there, and everyone is done with the one before it
         const int j0 = tiles.tile(it) * KT;

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
     constexpr int KT = key_tile<T, DT, NW>(), TB = KT * L::RB, QT = 32 * NW;
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K tile, V tile]
+    __shared__ __attribute__((aligned(16))) char k0[TB], k1[TB], v0[TB], v1[TB];       // apart, so that loads into one hold up no reads of another
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
     const int item = (int)xcd_item(blockIdx.x, gridDim.x);
     const int qt = item % a.nqt, bh = item / a.nqt, b = bh / a.Hk, hk = bh - b * a.Hk;
@@ -79,12 +79,12 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
     const int flo = max(wp1 - a.view.left, 0), fhi = min(wp0 + a.view.right, len - 1);
 
     const T *kp = (const T *)a.k + b * a.kb + hk * a.kh, *vp = (const T *)a.v + b * a.vb + hk * a.vh;
-    Stage<T, DT, KT, 64 * NW> sk, sv;
+    Direct<T, DT, KT, 64 * NW> sk, sv;
     sk.strided(a.kn);
     sv.strided(a.vn);
-    auto fetch = [&](int t) {
-        sk.fetch(kp + (long)t * KT * a.kn, len - t * KT, a.D);
-        sv.fetch(vp + (long)t * KT * a.vn, len - t * KT, a.D);
+    auto fetch = [&](int t, char *ks, char *vs) __attribute__((always_inline)) {
+        sk.fetch(ks, kp + (long)t * KT * a.kn, len - t * KT, a.D);
+        sv.fetch(vs, vp + (long)t * KT * a.vn, len - t * KT, a.D);
     };
 
     pa_f16v dq[DT / 32];
@@ -92,29 +92,26 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
     for (int ct = 0; ct < DT / 32; ++ct) dq[ct] = (pa_f16v)(0.f);
 
     const TileList<KT> tiles(a.view, start + a.g.div(r0), start + a.g.div(min(r0 + QT, rows) - 1), len);
-    if (tiles.n) fetch(tiles.tile(0));
-    for (int it = 0; it < tiles.n; ++it) {
-        char *ks = smem + (it & 1) * 2 * TB, *vs = ks + TB;
-        sk.store(ks);
-        sv.store(vs);
-        __syncthreads();
+    if (tiles.n) fetch(tiles.tile(0), k0, v0);
+    auto step = [&](int it, char *ks, char *vs, char *kn, char *vn) __attribute__((always_inline)) {
+        arrived();
+        __syncthreads();                                       // the tile is there, and everyone is done with the one before it
         const int j0 = tiles.tile(it) * KT;
-        if (it + 1 < tiles.n) fetch(tiles.tile(it + 1));
-        if (!wave_on) continue;
+        if (it + 1 < tiles.n) fetch(tiles.tile(it + 1), kn, vn);
+        if (!wave_on) return;
 #pragma unroll
         for (int sub = 0; sub < KT / 32; ++sub) {
             const int js = j0 + sub * 32;
             if (!((js <= whi && js + 31 >= wlo) || js < min(a.view.sinks, whi + 1))) continue;
             pa_f16v s = (pa_f16v)(0.f), dp = (pa_f16v)(0.f);
 #pragma unroll
-            for (int kk = 0; kk < DT / 16; ++kk) {
-                mma(s, L::ld(ks, sub * 32, kk), qf[kk]);
-                mma(dp, L::ld(vs, sub * 32, kk), gf[kk]);
-            }
+            for (int kk = 0; kk < DT / 16; ++kk) mma(s, L::ld(ks, sub * 32, kk), qf[kk]);
             if (!(js >= flo && js + 31 <= fhi)) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = keys.sees(js + 8 * (r >> 2) + 4 * h + (r & 3)) ? s[r] : -INFINITY;
             }
+#pragma unroll
+            for (int kk = 0; kk < DT / 16; ++kk) mma(dp, L::ld(vs, sub * 32, kk), gf[kk]);              // meanwhile the exponentials
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = ex2(__builtin_fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
 #pragma unroll
@@ -124,6 +121,10 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
                 for (int ct = 0; ct < DT / 32; ++ct) mma(dq[ct], L::ldt(ks, sub * 32 + 16 * u, ct * 32), ds);
             }
         }
+    };
+    for (int it = 0; it < tiles.n; it += 2) {
+        step(it, k0, v0, k1, v1);
+        if (it + 1 < tiles.n) step(it + 1, k1, v1, k0, v0);
     }
     if (row >= rows) return;
     T *dp = (T *)a.dq + (((size_t)b * a.N + i) * a.H + hq) * a.D;
@@ -176,8 +177,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
 {
     typedef Tile<T, DT> L;
     typedef typename Frag<T>::type F;
-    constexpr int KB = 32 * NW, RT = row_tile<T, DT>(), TB = RT * L::RB, BUF = 2 * TB + 3 * RT * 4;
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][Q tile, dO tile, lse, delta, position]
+    constexpr int KB = 32 * NW, RT = row_tile<T, DT>(), TB = RT * L::RB;
+    __shared__ __attribute__((aligned(16))) char q0[TB], q1[TB], g0[TB], g1[TB];
+    __shared__ __attribute__((aligned(16))) float r0[3][RT], r1[3][RT];                // of the tile's rows: lse, delta, position
     const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, h = l >> 5;
     const Walk w(a, blockIdx.x, KB, NW);
     const int b = w.bh / a.Hk, hk = w.bh - b * a.Hk;
@@ -215,12 +217,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
 
     // A tile is a.rt rows: whole queries, so that a thread's rows have the same head and the same distance from the tile's first query every time.
     // (More than RT heads a group: RT rows from anywhere, decoded each time.)
-    Stage<T, DT, RT, 64 * NW> sq, sg;
+    Direct<T, DT, RT, 64 * NW> sq, sg;
     const bool whole = a.G <= RT;
     float pl = 0.f, pd = 0.f;
     int pp = 0;
     const T *qp = (const T *)a.q + b * a.qb + (long)hk * a.G * a.qh, *gp = (const T *)a.dout + b * a.gb + (long)hk * a.G * a.gh;
-    auto place = [&](int first) {                              // offsets of the tile's rows from query first / G
+    auto place = [&](int first) __attribute__((always_inline)) {                              // offsets of the tile's rows from query first / G
 #pragma unroll
         for (int u = 0; u < sq.N; ++u) {
             const int x = first + sq.row(u), i = a.g.div(x), g = x - i * a.G;
@@ -230,11 +232,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
     };
     place(0);
     const int li = a.g.div(tid), lg = hk * a.G + tid - li * a.G;       // row tid of a tile: query and head (threads below RT)
-    auto fetch = [&](int t) {
+    auto fetch = [&](int t, char *qs, char *gs) __attribute__((always_inline)) {
         const int first = ra + t * a.rt, i0 = a.g.div(first), valid = min(a.rt, rb - first);
         if (!whole) place(first - i0 * a.G);
-        sq.fetch(qp + (long)i0 * a.qn, valid, a.D);            // padding rows are behind rb
-        sg.fetch(gp + (long)i0 * a.gn, valid, a.D);
+        sq.fetch(qs, qp + (long)i0 * a.qn, valid, a.D);        // padding rows are behind rb
+        sg.fetch(gs, gp + (long)i0 * a.gn, valid, a.D);
         if (tid < RT) {
             int i = i0 + li, hq = lg;
             if (!whole) {
@@ -252,45 +254,47 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
 #pragma unroll
     for (int ct = 0; ct < DT / 32; ++ct) dk[ct] = dv[ct] = (pa_f16v)(0.f);
 
-    if (t0 < t1) fetch(t0);
-    for (int t = t0; t < t1; ++t) {
-        char *qs = smem + ((t - t0) & 1) * BUF, *gs = qs + TB;
-        float *ls = reinterpret_cast<float *>(gs + TB), *ds = ls + RT;
-        int *ps = reinterpret_cast<int *>(ds + RT);
-        sq.store(qs);
-        sg.store(gs);
+    if (t0 < t1) fetch(t0, q0, g0);
+    auto step = [&](int t, char *qs, char *gs, float (&rs)[3][RT], char *qn, char *gn) __attribute__((always_inline)) {
+        const float *ls = rs[0], *ds = rs[1];
+        const int *ps = reinterpret_cast<const int *>(rs[2]);
         if (tid < RT) {
-            ls[tid] = pl;
-            ds[tid] = pd;
-            ps[tid] = pp;
+            rs[0][tid] = pl;
+            rs[1][tid] = pd;
+            rs[2][tid] = __int_as_float(pp);
         }
+        arrived();
         __syncthreads();
-        if (t + 1 < t1) fetch(t + 1);
-        if (!wave_on) continue;
+        if (t + 1 < t1) fetch(t + 1, qn, gn);
+        if (!wave_on) return;
 #pragma unroll
         for (int sub = 0; sub < RT / 32; ++sub) {
-            const int rs = ra + t * a.rt + sub * 32, re = min(min(rs + 31, ra + t * a.rt + a.rt - 1), rb - 1);
-            if (rs > re || (w.far && (t * (RT / 32) + sub) % NW != wave)) continue;
-            const int p0 = start + a.g.div(rs), p1 = start + a.g.div(re);
+            const int rf = ra + t * a.rt + sub * 32, re = min(min(rf + 31, ra + t * a.rt + a.rt - 1), rb - 1);
+            if (rf > re || (w.far && (t * (RT / 32) + sub) % NW != wave)) continue;
+            const int p0 = start + a.g.div(rf), p1 = start + a.g.div(re);
             if (!(p1 >= wk - a.view.right && (p0 <= wk1 + a.view.left || wk < a.view.sinks))) continue;
             pa_f16v s = (pa_f16v)(0.f), dp = (pa_f16v)(0.f);
 #pragma unroll
-            for (int kk = 0; kk < DT / 16; ++kk) {
-                mma(s, L::ld(qs, sub * 32, kk), kf[kk]);
-                mma(dp, L::ld(gs, sub * 32, kk), vf[kk]);
+            for (int kk = 0; kk < DT / 16; ++kk) mma(s, L::ld(qs, sub * 32, kk), kf[kk]);
+            if (!(p0 >= wk + 31 - a.view.right && p1 <= wk + a.view.left && wk + 31 < len)) {           // some row does not see some key
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int4 pos = *reinterpret_cast<const int4 *>(ps + sub * 32 + 8 * u + 4 * h);
+                    const int pe[4] = {pos.x, pos.y, pos.z, pos.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[4 * u + e] = (u32)pe[e] - (u32)plo <= span ? s[4 * u + e] : -INFINITY;
+                }
             }
-            const bool full = p0 >= wk + 31 - a.view.right && p1 <= wk + a.view.left && wk + 31 < len;
+#pragma unroll
+            for (int kk = 0; kk < DT / 16; ++kk) mma(dp, L::ld(gs, sub * 32, kk), vf[kk]);              // meanwhile the exponentials
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int rr = sub * 32 + 8 * u + 4 * h;
                 const pa_f4 lse = *reinterpret_cast<const pa_f4 *>(ls + rr), delta = *reinterpret_cast<const pa_f4 *>(ds + rr);
-                const int4 pos = *reinterpret_cast<const int4 *>(ps + rr);
-                const int pe[4] = {pos.x, pos.y, pos.z, pos.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * u + e;
-                    const float p = ex2(__builtin_fmaf(s[r], a.c, -lse[e]));
-                    s[r] = full || (u32)pe[e] - (u32)plo <= span ? p : 0.f;
+                    s[r] = ex2(__builtin_fmaf(s[r], a.c, -lse[e]));
                     dp[r] = s[r] * (dp[r] - delta[e]);
                 }
             }
@@ -304,6 +308,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
                 }
             }
         }
+    };
+    for (int t = t0; t < t1; t += 2) {
+        step(t, q0, g0, r0, q1, g1);
+        if (t + 1 < t1) step(t + 1, q1, g1, r1, q0, g0);
     }
     if (w.far && j >= a.view.sinks) return;                     // nobody reads those
     if (w.slot >= 0) {
@@ -407,18 +415,14 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int 
 template <typename T, int DT, int NW>
 void launch_dq(const BwdArgs &a, hipStream_t st)
 {
-    constexpr int lds = 4 * key_tile<T, DT, NW>() * DT * (int)sizeof(T);
-    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&dq_kernel<T, DT, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    hipLaunchKernelGGL((dq_kernel<T, DT, NW>), dim3((unsigned)((long)a.nqt * a.B * a.Hk)), dim3(64 * NW), lds, st, a);
+    hipLaunchKernelGGL((dq_kernel<T, DT, NW>), dim3((unsigned)((long)a.nqt * a.B * a.Hk)), dim3(64 * NW), 0, st, a);
 }
 
 template <typename T, int DT, int NW>
 void launch_dkv(const BwdArgs &a, int joined, hipStream_t st)
 {
-    constexpr int RT = row_tile<T, DT>(), lds = 2 * (2 * RT * DT * (int)sizeof(T) + 3 * RT * 4);
-    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&dkv_kernel<T, DT, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     const long bh = (long)a.B * a.Hk;
-    hipLaunchKernelGGL((dkv_kernel<T, DT, NW>), dim3((unsigned)(bh * a.groups * a.fars + bh * a.nkt * a.slices)), dim3(64 * NW), lds, st, a);
+    hipLaunchKernelGGL((dkv_kernel<T, DT, NW>), dim3((unsigned)(bh * a.groups * a.fars + bh * a.nkt * a.slices)), dim3(64 * NW), 0, st, a);
     if (joined) hipLaunchKernelGGL((dkv_join_kernel<T, DT, NW>), dim3((unsigned)(bh * joined * 32 * NW)), dim3(256), 0, st, a, joined);
 }
 
