@@ -9,6 +9,8 @@
 // 16 u + 8 + 4 h + e - 4: a product computed into registers feeds the next one without leaving them, if the other operand lists its contraction
 // index in the same order (ldt below).
 #pragma once
+#include <initializer_list>
+
 #include "pa_common.h"
 
 typedef float pa_f16v __attribute__((ext_vector_type(16)));
@@ -36,10 +38,6 @@ __device__ __forceinline__ long xcd_item(long x, long n)
     const long k = x & 7, each = n >> 3, rest = n & 7;
     return k * each + (k < rest ? k : rest) + (x >> 3);
 }
-
-template <int X> struct Const {
-    __device__ constexpr int operator()() const { return X; }
-};
 
 template <typename T> struct Frag;
 template <> struct Frag<float> { typedef pa_f8 type; };
@@ -294,6 +292,15 @@ static inline int window_attention_check(const char *name, int dtype, int b, int
                right, sinks);
     PA_REQUIRE(scale > 0.f && scale < INFINITY, "%s: the scale has to be positive and finite", name);
     return PA_OK;
+}
+
+// largest power of two up to 16 that divides every address and every stride (in bytes)
+static inline long alignment_of(int es, std::initializer_list<const void *> ps, std::initializer_list<long> ss)
+{
+    unsigned long m = 16;
+    for (const void *p : ps) m |= (unsigned long)(uintptr_t)p;
+    for (long s : ss) m |= (unsigned long)(s * es);
+    return (long)(m & -m);
 }
 
 // a tile's rows are addressed by 32-bit offsets: 64 tokens and 64 heads of 4-byte elements stay below 2^32 bytes

@@ -260,7 +260,6 @@ template <typename T, int DT>
 int launch_paged(const PagedArgs &a, hipStream_t st)
 {
     constexpr int lv = 4 * KT * DT * (int)sizeof(T), lj = (32 * (DT + 4) + 256) * 4, lds = lv > lj ? lv : lj;
-    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_kernel<T, DT>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     hipLaunchKernelGGL((paged_kernel<T, DT>), dim3((unsigned)((long)a.B * a.Hk * a.ngt), (unsigned)a.runs), dim3(256), lds, st, a);
     if (a.runs > 1) {
         const long threads = (long)a.B * a.H * (DT / 4);
@@ -318,6 +317,8 @@ PA_API int pa_paged_attention(int dtype, int b, int h, int hk, int d, const void
     PA_REQUIRE(scale > 0.f && scale < INFINITY, "pa_paged_attention: the scale has to be positive and finite");
     if (b == 0) return PA_OK;
     PA_REQUIRE(q && out && length && (width_ == 0 || table) && (pages == 0 || (k_pages && v_pages)), "pa_paged_attention: null tensor");
+    PA_REQUIRE(alignment_of(dtype == PA_DT_F32 ? 4 : 2, {q, k_pages, v_pages, out, scratch}, {qb, qh, kp, kt, kh, vp, vt, vh}) == 16,
+               "pa_paged_attention: addresses and strides have to be multiples of 16 bytes");
     PagedArgs a;
     a.q = q; a.k = k_pages; a.v = v_pages; a.table = table; a.length = length; a.out = out; a.part = scratch;
     a.qb = qb; a.qh = qh; a.kp = kp; a.kt = kt; a.kh = kh; a.vp = vp; a.vt = vt; a.vh = vh; a.tb = width_;
@@ -350,6 +351,8 @@ PA_API int pa_paged_append(int dtype, int b, int tokens, int hk, int d, const vo
     if (b == 0 || tokens == 0 || pages == 0 || width_ == 0) return PA_OK;
     PA_REQUIRE(k && v && k_pages && v_pages && table && starts, "pa_paged_append: null tensor");
     const int es = dtype == PA_DT_F32 ? 4 : 2, chunks = d * es / 16;
+    PA_REQUIRE(alignment_of(es, {k, v, k_pages, v_pages}, {kb, kn, kh, vb, vn, vh, kp, kt, kph, vp, vt, vph}) == 16,
+               "pa_paged_append: addresses and strides have to be multiples of 16 bytes");
     const long total = (long)b * tokens * hk * chunks;
     PA_REQUIRE((total + 255) / 256 < (1l << 31), "pa_paged_append: too many workgroups");
     hipLaunchKernelGGL(append_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, total, tokens, hk, chunks, es, (const char *)k,

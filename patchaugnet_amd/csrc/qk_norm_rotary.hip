@@ -13,8 +13,6 @@
 //
 // The weight gradients are sums over all tokens and heads: per lane in registers over a workgroup's tokens, then across the workgroup, then by a
 // second launch over the workgroups' rows, always in the same order.
-#include <initializer_list>
-
 #include "pa_attn.h"
 
 using pa_attn::Div;
@@ -390,15 +388,6 @@ int norm_plan(NormArgs &a, int dtype, int b, bool bwd, long mask)
 
 }  // namespace
 
-// q (b, n, h, d) and k (b, n, hk, d) with strides in elements, unit stride in d; mask: the bitwise or of every address and of every stride in bytes
-static long mask_of(int es, std::initializer_list<const void *> ps, std::initializer_list<long> ss)
-{
-    unsigned long m = 16;
-    for (const void *p : ps) m |= (unsigned long)(uintptr_t)p;
-    for (long s : ss) m |= (unsigned long)(s * es);
-    return (long)(m & -m);                                      // largest power of two that divides all of them
-}
-
 PA_API int pa_qk_norm_rotary(int dtype, int b, int n, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn, long kh,
                              const void *qw, const void *kw, int w_f32, const void *pos, int ptype, long pb, const float *freq, int axes, int per, float eps,
                              int interleaved, void *q_out, void *k_out, pa_stream_t stream)
@@ -413,7 +402,7 @@ PA_API int pa_qk_norm_rotary(int dtype, int b, int n, int h, int hk, int d, cons
     a.pos = pos; a.freq = freq; a.pb = pb;
     a.N = n; a.D = d; a.axes = axes; a.per = per; a.interleaved = interleaved; a.wtype = w_f32; a.ptype = ptype; a.eps = eps;
     const int es = dtype == F32 ? 4 : 2;
-    const int v = norm_plan(a, dtype, b, false, mask_of(es, {q, k, q_out, k_out}, {qb, qn, qh, kb, kn, kh, d}));
+    const int v = norm_plan(a, dtype, b, false, alignment_of(es, {q, k, q_out, k_out}, {qb, qn, qh, kb, kn, kh, d}));
     const long groups = (a.tokens + a.tb - 1) / a.tb;
     PA_REQUIRE(groups < (1l << 31), "pa_qk_norm_rotary: too many workgroups");
     const size_t lds = (size_t)2 * a.tb * a.pairs * 4;
@@ -443,7 +432,7 @@ PA_API int pa_qk_norm_rotary_backward(int dtype, int b, int n, int h, int hk, in
     a.N = n; a.D = d; a.axes = axes; a.per = per; a.interleaved = interleaved; a.wtype = w_f32; a.ptype = ptype; a.eps = eps;
     a.part = dqw || dkw ? scratch : nullptr;
     const int es = dtype == F32 ? 4 : 2;
-    const int v = norm_plan(a, dtype, b, true, mask_of(es, {q, k, gq, gk, dq, dk}, {qb, qn, qh, kb, kn, kh, gqb, gqn, gqh, gkb, gkn, gkh, d}));
+    const int v = norm_plan(a, dtype, b, true, alignment_of(es, {q, k, gq, gk, dq, dk}, {qb, qn, qh, kb, kn, kh, gqb, gqn, gqh, gkb, gkn, gkh, d}));
     const int groups = groups_of(a.tokens, a.tb);
     size_t lds = (size_t)2 * a.tb * a.pairs * 4;
     if (lds < (size_t)2 * d * 4) lds = (size_t)2 * d * 4;

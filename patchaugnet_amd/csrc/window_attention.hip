@@ -245,6 +245,8 @@ PA_API int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, in
     if (rc != PA_OK) return rc;
     if (b == 0 || n == 0) return PA_OK;
     PA_REQUIRE(q && out && (m == 0 || (k && v)), "pa_window_attention: null tensor");
+    PA_REQUIRE(alignment_of(dtype == PA_DT_F32 ? 4 : 2, {q, k, v, out}, {qb, qn, qh, kb, kn, kh, vb, vn, vh}) == 16,
+               "pa_window_attention: addresses and strides have to be multiples of 16 bytes");
     FwdArgs a;
     a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.part = scratch;
     a.qb = qb; a.qn = qn; a.qh = qh; a.kb = kb; a.kn = kn; a.kh = kh; a.vb = vb; a.vn = vn; a.vh = vh;

@@ -462,6 +462,8 @@ PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, i
     if (rc != PA_OK) return rc;
     if (b == 0 || (n == 0 && m == 0)) return PA_OK;
     PA_REQUIRE((n == 0 || (q && out && lse && dout && dq && scratch)) && (m == 0 || (k && v && dk && dv)), "pa_window_attention_backward: null tensor");
+    PA_REQUIRE(alignment_of(dtype == PA_DT_F32 ? 4 : 2, {q, k, v, out, dout, dq, dk, dv, scratch}, {qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh}) == 16,
+               "pa_window_attention_backward: addresses and strides have to be multiples of 16 bytes");
     BwdArgs a;
     a.q = q; a.k = k; a.v = v; a.out = out; a.dout = dout; a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv;
     a.delta = scratch;

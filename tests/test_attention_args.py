@@ -87,3 +87,19 @@ def test_scratch_is_bounded(lib):
     assert 0 < g(1, 16, 16384, 8, 8, 64, -1, 0, 0) <= 64 * 16 * 8 * (64 + 2)
     assert w(1, 64, 64, 8, 8, 64, -1, 0, 0) >= 64 * 8
     assert f(0, 8, 2, 64, 16, 7, -1, 0) == 0 and g(1, 0, 4, 2, 1, 32, 0, 0, 0) == 0
+
+
+def test_misaligned_addresses_are_refused(lib):
+    """Rows that do not start at multiples of 16 bytes (host addresses: the call ends before anything is launched)."""
+    buf = (ctypes.c_char * 4096)()
+    base = (ctypes.addressof(buf) + 15) // 16 * 16
+    p, z = ctypes.c_void_p(0), (ctypes.c_void_p(base), 0, 32, 32)
+    at, off = ctypes.c_void_p(base), (ctypes.c_void_p(base + 8), 0, 32, 32)
+    skew = (ctypes.c_void_p(base), 0, 34, 32)
+    for bad in (off, skew):
+        assert lib.pa_window_attention(0, 1, 1, 1, 1, 1, 32, *bad, *z, *z, -1, 0, 0, 1.0, p, p, at, p, at, p) == -1
+        assert b"16 bytes" in lib.pa_last_error()
+        assert lib.pa_window_attention_backward(0, 1, 1, 1, 1, 1, 32, *z, *bad, *z, at, at, *z, -1, 0, 0, 1.0, p, p, at, at, at, at, p) == -1
+        assert lib.pa_paged_attention(0, 1, 1, 1, 32, at, 0, 32, *bad, *z, 1, 1, at, 1, at, -1, 0, 1.0, at, at, p) == -1
+        assert lib.pa_paged_append(0, 1, 1, 1, 32, *bad, *z, *z, *z, 1, 1, at, 1, at, p, p) == -1
+        assert b"16 bytes" in lib.pa_last_error()

@@ -238,3 +238,18 @@ def test_refusals():
     (g,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), leaf)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (F16, 64), (BF16, 96), (F32, 128), (F32, 64)])
+@pytest.mark.parametrize("H,Hk", [(4, 1), (3, 1), (2, 2)])
+def test_rows_far_behind_the_first_tokens(dtype, D, H, Hk):
+    """Many rows that see the first tokens only beyond their window: those gradients are gathered apart and joined.  Two groups of 32 first tokens."""
+    _check(*_qkv(1, 900, 900, H, Hk, D, dtype, seed=D + H), 100, 0, 37)
+    _check(*_qkv(2, 700, 700, H, Hk, D, dtype, seed=D), 300, 20, 5, lengths=[700, 411])
+
+
+@pytest.mark.parametrize("H,Hk", [(5, 1), (7, 1), (24, 1), (64, 1), (65, 1), (130, 1)])
+def test_large_groups(H, Hk):
+    """Groups that do not divide a tile of rows, fill one, and exceed one."""
+    _check(*_qkv(1, 60, 60, H, Hk, 32, BF16, seed=H), 11, 4, 2)
+    _check(*_qkv(1, 40, 40, H, Hk, 128, F32, seed=H), 11, 0, 1)
