@@ -23,7 +23,6 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call
 
 __all__ = ["qk_norm_rotary", "window_attention", "paged_append", "paged_attention"]
 
@@ -44,7 +43,7 @@ def _check(name, *tensors):
             raise RuntimeError(f"{name} runs on the MI355X only: got a tensor on {t.device} (there is no CPU form)")
         if t.dtype != first.dtype:
             raise TypeError(f"{name}: tensors of one type; got {[x.dtype for x in tensors]}")
-        if t.device != first.device:
+        if t.get_device() != first.get_device():
             raise RuntimeError(f"{name}: tensors on {first.device} and {t.device}")
     dt = _DTYPE.get(first.dtype)
     if dt is None:
@@ -61,7 +60,7 @@ def _ints(name, what, t, device, n):
     """A (n,) int32 device vector or None."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != n:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.get_device() != device.index or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name}: {what} has to be an int32 tensor of shape ({n},) on {device}")
     return t.contiguous()
 
@@ -121,6 +120,19 @@ def _scale(name, scale, D):
 
 def ptr(t):
     return t.data_ptr() if t is not None else None
+
+
+_entry = {}
+
+
+def call(name, *args):
+    """An entry point on the current stream of the current device; raises what the library says."""
+    f = _entry.get(name)
+    if f is None:
+        f = _entry[name] = getattr(_lib.lib(), name)
+    rc = f(*args, _lib.stream_ptr())
+    if rc:
+        raise RuntimeError(f"{name} failed ({rc}): {_lib.lib().pa_last_error().decode()}")
 
 
 @functools.lru_cache(maxsize=256)
