@@ -8,6 +8,7 @@ Layout:
   pt_util.py, loupe.py, backbone.py, patch_aug_net.py, pptnet.py
                    model classes with the reference's API and state-dict keys
   engine.py        fused inference engine (eval mode)
+  attention.py     norm + rotation, windowed attention and its paged one-token form over ordered tokens
   weights.py, configs.py  deterministic weights / synthetic submaps, hot-path hyper-parameters
 """
 __version__ = "0.1.0"

@@ -332,7 +332,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, starts, *, counts=None):
 
     Token t < counts[b] (None: T) of sequence b goes to position starts[b] + t: row position % page of page page_table[b, position // page].  int32
     tables.  Positions outside the table and entries outside the pool (-1, ...) are skipped; everything else in the pool stays as it is.  Two
-    tokens for one row of one page leave either of them, in parts."""
+    tokens for one row of one page leave either of them, in parts; k and v must not lie in the pools."""
     name = "paged_append"
     dt = _check(name, k, v, k_pages, v_pages)
     _no_gradient(name, k, v, k_pages, v_pages)

@@ -10,6 +10,10 @@
 // lane pair straight from memory as the operand of S^T = K Q^T (Q: the heads that share the key head, up to 32 rows), and V goes through 32 rows of
 // LDS of its own to be read transposed.  The next tile is requested before the present one is used.  Waves join in LDS, runs in a second launch --
 // none when one run covers the cache.
+//
+// Measured: 48 sequences of 4096 to 16384 tokens, 32 heads of 128 over 8, bf16, pages of 64: 381 + 7 us for 1.95 GB = 5.0 TB/s (a 2 GiB copy: 4.9, read and
+// written).  With one wave per SIMD (290 registers) and a branch around every load it was 525 us.  100 tokens, 8 heads of 64 over 2: 5.3 us, one launch.
+// append: 16 prompts of up to 2048 tokens, 8 heads of 128: 147 MB in 25 us = 5.9 TB/s; one token of 32 sequences 3.2 us.
 #include "pa_attn.h"
 
 using namespace pa_attn;

@@ -11,6 +11,11 @@
 // expensive part (64-bit range reduction: positions of 10^6 keep full accuracy); a workgroup computes those of its tokens once, into LDS, for all
 // query and key heads.  Everything between load and store is 32-bit, rounded once.
 //
+// Measured, forward / backward / weights: bf16 8 x 4096 tokens, 16 + 4 heads of 128: 75 / 129 / 5 us (336 and 503 MB: 4.5 and 3.9 TB/s; a copy: 4.9);
+// float32 18 x 1024, 8 + 8 heads of 64, three axes: 28 / 47 / 4 us.  Addresses and angles once per token (64-bit products per row cost 224 us backward),
+// the next row in flight.  The width of a piece is 16 bytes, and less where the number of pairs is not a multiple of it: an odd number (34 of 96
+// elements rotated) means 2-byte pieces and 1 TB/s.
+//
 // The weight gradients are sums over all tokens and heads: per lane in registers over a workgroup's tokens, then across the workgroup, then by a
 // second launch over the workgroups' rows, always in the same order.
 #include "pa_attn.h"

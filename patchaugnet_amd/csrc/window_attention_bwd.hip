@@ -14,6 +14,11 @@
 //
 // Roundings: P and dS are rounded to the operand type for the second products (16-bit types); the scale is applied to the 32-bit sums, so that dS is
 // rounded before it gets smaller.
+//
+// Measured, dq / dk and dv / join: bf16 4 x 4096 tokens, 16 heads of 64 over 4, window 512: 77 / 113 / 5 us (630 / 575 TFLOP/s of visible pairs); all keys of
+// 4 x 2048, 16 heads of 64: 114 / 157 us (900 / 870; a library product: 1219); 2 x 8192, 16 of 128 over 4, window 1024: 215 / 466 / 7 us; float32
+// 18 x 1024, 8 heads of 32, 128 keys either side: 122 / 158 / 9 us.  Bound by MFMA and LDS reads together (16 KB read for 16 to 32 products of a wave).
+// dk, dv at width 128 holds 390 registers, one wave per SIMD: there nothing hides a wave's exponentials, and its rate is 550.
 #include "pa_attn.h"
 
 using namespace pa_attn;
@@ -388,7 +393,7 @@ struct Shape {
 
 // Slices: keys that do not fill the chip (fewer than 2048 waves, two per SIMD) have their walks cut, each slice with at least four row tiles;
 // far rows are cut into slices of
-// 16 row tiles.
+// 16 row tiles, more where the slices alone would fill the chip several times (2048 of them).
 Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int right, int sinks, bool started)
 {
     Shape s;
@@ -407,7 +412,9 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int 
     const bool far = first > 0 && (started ? left < M : left < N - 1);          // rows behind the window of the first tokens
     s.groups = far ? pa_div_up(first, 32) : 0;
     s.nst = pa_div_up(first, kb);
-    const long f = (rows + 16 * s.rt - 1) / (16 * s.rt);
+    long f = (rows + 16 * s.rt - 1) / (16 * s.rt);
+    const long most = s.groups ? 2048 / (bh * s.groups) : 0;
+    f = f > most ? most : f;
     s.fars = far ? (f > 64 ? 64 : f < 1 ? 1 : (int)f) : 1;
     return s;
 }

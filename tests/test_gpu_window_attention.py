@@ -253,3 +253,24 @@ def test_large_groups(H, Hk):
     """Groups that do not divide a tile of rows, fill one, and exceed one."""
     _check(*_qkv(1, 60, 60, H, Hk, 32, BF16, seed=H), 11, 4, 2)
     _check(*_qkv(1, 40, 40, H, Hk, 128, F32, seed=H), 11, 0, 1)
+
+
+def test_keys_behind_four_gigabytes():
+    """Keys and values of more than 2^31 elements: the last queries see the last keys and the first ones; all other gradients are zero."""
+    M, N, D, left, sinks = 2 ** 24 + 40, 40, 128, 100, 3
+    g = torch.Generator(device="cuda").manual_seed(12)
+    q, do = (torch.randn(1, N, 2, D, generator=g, device="cuda").to(BF16) for _ in range(2))
+    k, v = (torch.zeros(1, M, 1, D, dtype=BF16, device="cuda") for _ in range(2))
+    near = torch.cat([torch.arange(sinks), torch.arange(M - N - left - 8, M)]).cuda()
+    for t in (k, v):
+        t[0, near] = torch.randn(near.numel(), 1, D, generator=g, device="cuda").to(BF16)
+    got = _run(q, k, v, do, left, 0, sinks, lengths=[M], starts=[M - N])
+    # the same rows over the keys that hold anything: the first ones, then the last ones, which keep their distances to the queries
+    ks, vs = k[:, near], v[:, near]
+    m = near.numel()
+    val, tol = reference(q, ks, vs, left, 0, sinks, None, [m], [m - N], do)
+    for n in ("out", "dq"):
+        close(got[n], val[n], tol[n], n)
+    for n in ("dk", "dv"):
+        close(got[n][:, near], val[n], tol[n], n)
+        assert int(got[n].count_nonzero()) == int(got[n][:, near].count_nonzero())
