@@ -273,8 +273,9 @@ static inline int waves_of(int es, long reach) { return es == 4 || reach < 256 ?
 // waves on a SIMD that the registers are held down to
 template <typename T, int DT> constexpr int waves_per_simd() { return sizeof(T) == 2 ? 2 : DT <= 32 ? 3 : DT <= 64 ? 2 : 1; }
 
-// Keys of a tile of the kernels that own rows: fewer where two waves alone bring wide rows into LDS (registers).
-template <typename T, int DT, int NW> constexpr int key_tile() { return NW == 2 && DT * (int)sizeof(T) >= 256 ? 32 : 64; }
+// Keys of a tile of the kernels that own rows: two-wave workgroups with 64 keys would fill the LDS before the registers (float32 18 x 1024, 8 heads of 32,
+// 128 keys either side: forward 88 us, dq 121; with 32 keys 76 and 109).
+template <typename T, int DT, int NW> constexpr int key_tile() { return NW == 2 ? 32 : 64; }
 
 static inline int width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }      // padded head width
 

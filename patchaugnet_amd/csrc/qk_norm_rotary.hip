@@ -13,8 +13,8 @@
 //
 // Measured, forward / backward / weights: bf16 8 x 4096 tokens, 16 + 4 heads of 128: 75 / 129 / 5 us (336 and 503 MB: 4.5 and 3.9 TB/s; a copy: 4.9);
 // float32 18 x 1024, 8 + 8 heads of 64, three axes: 28 / 47 / 4 us.  Addresses and angles once per token (64-bit products per row cost 224 us backward),
-// the next row in flight.  The width of a piece is 16 bytes, and less where the number of pairs is not a multiple of it: an odd number (34 of 96
-// elements rotated) means 2-byte pieces and 1 TB/s.
+// the next row in flight.  A piece is 16 bytes wide; where the number of pairs is no multiple of that, lanes keep pieces of consecutive elements and the
+// pairs are exchanged through LDS (2.0 to 3.5 TB/s); where the rows themselves do not start at 16 bytes, pieces are narrower (heads of 66: 0.7 TB/s).
 //
 // The weight gradients are sums over all tokens and heads: per lane in registers over a workgroup's tokens, then across the workgroup, then by a
 // second launch over the workgroups' rows, always in the same order.
@@ -43,6 +43,7 @@ struct NormArgs {
     float *part;                        // (workgroups, 2, D) partial weight gradients
     long pb;
     int tokens, N, D, axes, per, pairs, interleaved, wtype, ptype;
+    int exchange, pitch;                // pairs exchanged through LDS; angles of a token in LDS
     int tb, units, lpr;                 // tokens of a workgroup's turn, units of a row, lanes of a row (a power of two)
     float eps;
     Div dn, dpairs, dper;
@@ -91,13 +92,13 @@ template <typename T, int V> __device__ __forceinline__ void store(T *p, const f
 }
 
 // A row as units of two V-element pieces: the pairs' two halves, then the unrotated rest.  The last piece of an odd rest does not exist (V = 1 only).
-template <int V> struct Unit {
+template <int V, bool EX> struct Unit {
     int o1, o2, pair;                   // pair < 0: not rotated
     bool on, two;
 
     __device__ __forceinline__ Unit(const NormArgs &a, int u)
     {
-        const int rot = a.pairs / V;
+        const int rot = EX ? 0 : a.pairs / V;
         on = u < a.units;
         pair = u < rot ? u * V : -1;
         if (u < rot && !a.interleaved) {
@@ -111,7 +112,7 @@ template <int V> struct Unit {
     }
 };
 
-template <int V> __device__ __forceinline__ void rotate(float *x, const Unit<V> &t, int interleaved, const float *cs, const float *sn, float sign)
+template <int V> __device__ __forceinline__ void rotate(float *x, const Unit<V, false> &t, int interleaved, const float *cs, const float *sn, float sign)
 {
     if (t.pair < 0) return;
     if (interleaved) {
@@ -131,6 +132,35 @@ template <int V> __device__ __forceinline__ void rotate(float *x, const Unit<V> 
     }
 }
 
+// Place of element (or pair) e in LDS: lanes read 2 V apart, the skip spreads them over the banks.
+__device__ __forceinline__ int skip(int e) { return e + (e >> 4); }
+
+// The rotation where the pairs' second halves do not start at a whole piece: lanes keep pieces of consecutive elements, every element's partner comes
+// through the row's place in LDS.  A row is a wave's own, so LDS serves its stores and loads in order.
+template <int V> __device__ __forceinline__ void exchange(float *x, const Unit<V, true> &t, const NormArgs &a, float *row, const float *cs, const float *sn, float sign)
+{
+    int e0 = t.o1;
+    asm volatile("" : "+v"(e0));                                // the places are worked out here, not kept for 2 V elements over all rows
+    if (t.on) {
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) row[skip(e0 + i)] = x[i];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (t.on) {
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) {
+            const int e = e0 + i;
+            const bool first = a.interleaved ? (e & 1) == 0 : e < a.pairs;
+            const int other = a.interleaved ? e ^ 1 : first ? e + a.pairs : e - a.pairs, p = a.interleaved ? e >> 1 : first ? e : other;
+            if (e < 2 * a.pairs) {
+                const float y = row[skip(other)], c = cs[skip(p)], s = sign * sn[skip(p)];
+                x[i] = first ? x[i] * c - y * s : y * s + x[i] * c;
+            }
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 // 1 / sqrt(x): v_rsq_f32 and a Newton step; it flushes subnormal arguments, so small ones are lifted first
 __device__ __forceinline__ float rsqrt32(float x)
 {
@@ -143,8 +173,8 @@ __device__ __forceinline__ float rsqrt32(float x)
 
 // The rows of one side in a workgroup's turn of nt tokens from t0: row slot by row slot, the next one fetched while this one is computed.  where:
 // offsets of the turn's tokens in x and in g; cos, sin: their angles.  acc: this lane's sums for the weights' gradient.
-template <typename T, int V, int UPL, bool BWD>
-__device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int t0, int nt, const long *where, const float *cos, const float *sin,
+template <typename T, int V, int UPL, bool BWD, bool EX>
+__device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int t0, int nt, const long *where, const float *cos, const float *sin, float *mine,
                                           const float (&w)[UPL][2 * V], float (&acc)[BWD ? UPL : 1][2 * V])
 {
     typedef typename Vec<T, V>::type P;
@@ -162,7 +192,7 @@ __device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int
         r.y = (T *)sd.y + ((long)t0 * sd.heads + row) * a.D;
 #pragma unroll
         for (int p = 0; p < UPL; ++p) {
-            const Unit<V> t(a, lane + p * a.lpr);
+            const Unit<V, EX> t(a, lane + p * a.lpr);
             r.x[p][0] = r.x[p][1] = 0;
             if (t.on) r.x[p][0] = *reinterpret_cast<const P *>(x + t.o1);
             if (t.two) r.x[p][1] = *reinterpret_cast<const P *>(x + t.o2);
@@ -177,7 +207,7 @@ __device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int
     for (int row = slot; row < rows; row += slots) {
         if (row + slots < rows) fetch(nxt, row + slots);
         float v[UPL][2 * V], gr[BWD ? UPL : 1][2 * V], ss = 0.f;
-        const float *cs = cos + cur.tok * a.pairs, *sn = sin + cur.tok * a.pairs;
+        const float *cs = cos + cur.tok * a.pitch, *sn = sin + cur.tok * a.pitch;
 #pragma unroll
         for (int p = 0; p < UPL; ++p)
 #pragma unroll
@@ -191,10 +221,11 @@ __device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int
         if (!BWD) {
 #pragma unroll
             for (int p = 0; p < UPL; ++p) {
-                const Unit<V> t(a, lane + p * a.lpr);
+                const Unit<V, EX> t(a, lane + p * a.lpr);
 #pragma unroll
                 for (int i = 0; i < 2 * V; ++i) v[p][i] = v[p][i] * r * w[p][i];
-                rotate<V>(v[p], t, a.interleaved, cs, sn, 1.f);
+                if constexpr (EX) exchange<V>(v[p], t, a, mine, cs, sn, 1.f);
+                else rotate<V>(v[p], t, a.interleaved, cs, sn, 1.f);
                 if (t.on) store<T, V>(cur.y + t.o1, &v[p][0]);
                 if (t.two) store<T, V>(cur.y + t.o2, &v[p][V]);
             }
@@ -202,8 +233,9 @@ __device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int
             float dot = 0.f;
 #pragma unroll
             for (int p = 0; p < UPL; ++p) {
-                const Unit<V> t(a, lane + p * a.lpr);
-                rotate<V>(gr[p], t, a.interleaved, cs, sn, -1.f);
+                const Unit<V, EX> t(a, lane + p * a.lpr);
+                if constexpr (EX) exchange<V>(gr[p], t, a, mine, cs, sn, -1.f);
+                else rotate<V>(gr[p], t, a.interleaved, cs, sn, -1.f);
 #pragma unroll
                 for (int i = 0; i < 2 * V; ++i) {
                     v[p][i] *= r;                               // n
@@ -216,7 +248,7 @@ __device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int
             dot *= inv_d;
 #pragma unroll
             for (int p = 0; p < UPL; ++p) {
-                const Unit<V> t(a, lane + p * a.lpr);
+                const Unit<V, EX> t(a, lane + p * a.lpr);
 #pragma unroll
                 for (int i = 0; i < 2 * V; ++i) gr[p][i] = r * __builtin_fmaf(-v[p][i], dot, gr[p][i]);
                 if (t.on) store<T, V>(cur.y + t.o1, &gr[p][0]);
@@ -228,16 +260,17 @@ __device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int
 }
 
 // UPL: units a lane can hold (1 for the wide pieces, up to 4 for the narrow ones: 64 lanes x 4 units x 2 elements = MAXD)
-template <typename T, int V, int UPL, bool BWD>
+template <typename T, int V, int UPL, bool BWD, bool EX>
 __global__ __launch_bounds__(256, BWD ? 3 : 4) void norm_kernel(const NormArgs a)
 {
-    extern __shared__ __attribute__((aligned(16))) float sh[];       // [tb][pairs] cosines, [tb][pairs] sines; backward: then the join of 2 D sums
+    extern __shared__ __attribute__((aligned(16))) float sh[];       // [tb][pitch] cosines, [tb][pitch] sines, exchanges; backward: then the join of 2 D sums
     __shared__ long where[2][2][MAXTOK];
     const int tid = threadIdx.x, lane = tid & (a.lpr - 1);
+    float *mine = sh + 2 * a.tb * a.pitch + tid / a.lpr * (skip(a.D) + 1);       // this row slot's place for exchanges
     float w[2][UPL][2 * V], acc[2][BWD ? UPL : 1][2 * V];
 #pragma unroll
     for (int p = 0; p < UPL; ++p) {
-        const Unit<V> t(a, lane + p * a.lpr);
+        const Unit<V, EX> t(a, lane + p * a.lpr);
 #pragma unroll
         for (int i = 0; i < 2 * V; ++i) {
             const int e = (i < V ? t.o1 + i : t.o2 + i - V);
@@ -260,12 +293,13 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void norm_kernel(const NormArgs a
         for (int i = tid; i < nt * a.pairs; i += 256) {
             const int tok = a.dpairs.div(i), pr = i - tok * a.pairs, at = t0 + tok, b = a.dn.div(at);
             const float2 cs = turn(position_at(a, b, at - b * a.N, a.dper.div(pr)) * (double)a.freq[pr]);
-            sh[tok * a.pairs + pr] = cs.x;
-            sh[(a.tb + tok) * a.pairs + pr] = cs.y;
+            const int at_pr = tok * a.pitch + (EX ? skip(pr) : pr);
+            sh[at_pr] = cs.x;
+            sh[a.tb * a.pitch + at_pr] = cs.y;
         }
         __syncthreads();
-        side_rows<T, V, UPL, BWD>(a, a.side[0], t0, nt, where[0][0], sh, sh + a.tb * a.pairs, w[0], acc[0]);
-        side_rows<T, V, UPL, BWD>(a, a.side[1], t0, nt, where[1][0], sh, sh + a.tb * a.pairs, w[1], acc[1]);
+        side_rows<T, V, UPL, BWD, EX>(a, a.side[0], t0, nt, where[0][0], sh, sh + a.tb * a.pitch, mine, w[0], acc[0]);
+        side_rows<T, V, UPL, BWD, EX>(a, a.side[1], t0, nt, where[1][0], sh, sh + a.tb * a.pitch, mine, w[1], acc[1]);
     }
     if (!BWD || a.part == nullptr) return;
     // sums of this workgroup: over the rows of a wave by exchanges, over the waves through LDS
@@ -282,7 +316,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void norm_kernel(const NormArgs a
         if ((tid >> 6) == w && (tid & 63) < a.lpr) {
 #pragma unroll
             for (int p = 0; p < UPL; ++p) {
-                const Unit<V> t(a, lane + p * a.lpr);
+                const Unit<V, EX> t(a, lane + p * a.lpr);
 #pragma unroll
                 for (int i = 0; i < 2 * V; ++i) {
                     const int e = (i < V ? t.o1 + i : t.o2 + i - V);
@@ -324,13 +358,13 @@ __global__ __launch_bounds__(1024) void weight_kernel(const float *__restrict__ 
     }
 }
 
-// widest piece that every row start and every piece of a row is a multiple of
-int piece(int dtype, int d, int pairs, long mask)
+// Widest piece that every row start is a multiple of and a row (pairs: their two halves and the rest) consists of.
+int piece(int dtype, int d, int pairs, long align)
 {
     const int most = dtype == F32 ? 4 : 8;
     const long es = dtype == F32 ? 4 : 2;
     for (int v = most; v > 1; v >>= 1)
-        if (pairs % v == 0 && (d - 2 * pairs) % (2 * v) == 0 && mask % (v * es) == 0) return v;
+        if (pairs % v == 0 && (d - 2 * pairs) % (2 * v) == 0 && align % (v * es) == 0) return v;
     return 1;
 }
 
@@ -350,15 +384,22 @@ int turn_tokens(long tokens, int heads, int lpr, bool bwd)
 
 int groups_of(long tokens, int tb) { return (int)((tokens + tb - 1) / tb < MAXGROUPS ? (tokens + tb - 1) / tb : MAXGROUPS); }
 
+template <typename T, bool BWD, bool EX>
+void launch_pieces(const NormArgs &a, int v, dim3 grid, size_t lds, hipStream_t st)
+{
+    if constexpr (sizeof(T) == 2) {
+        if (v == 8) { hipLaunchKernelGGL((norm_kernel<T, 8, 1, BWD, EX>), grid, dim3(256), lds, st, a); return; }
+    }
+    if (v == 4) hipLaunchKernelGGL((norm_kernel<T, 4, 1, BWD, EX>), grid, dim3(256), lds, st, a);
+    else if (v == 2) hipLaunchKernelGGL((norm_kernel<T, 2, 2, BWD, EX>), grid, dim3(256), lds, st, a);
+    else if constexpr (!EX) hipLaunchKernelGGL((norm_kernel<T, 1, 4, BWD, EX>), grid, dim3(256), lds, st, a);
+}
+
 template <typename T, bool BWD>
 void launch_norm(const NormArgs &a, int v, dim3 grid, size_t lds, hipStream_t st)
 {
-    if constexpr (sizeof(T) == 2) {
-        if (v == 8) { hipLaunchKernelGGL((norm_kernel<T, 8, 1, BWD>), grid, dim3(256), lds, st, a); return; }
-    }
-    if (v == 4) hipLaunchKernelGGL((norm_kernel<T, 4, 1, BWD>), grid, dim3(256), lds, st, a);
-    else if (v == 2) hipLaunchKernelGGL((norm_kernel<T, 2, 2, BWD>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((norm_kernel<T, 1, 4, BWD>), grid, dim3(256), lds, st, a);
+    if (a.exchange) launch_pieces<T, BWD, true>(a, v, grid, lds, st);
+    else launch_pieces<T, BWD, false>(a, v, grid, lds, st);
 }
 
 int norm_check(const char *name, int dtype, int b, int n, int h, int hk, int d, int axes, int per, int ptype, float eps, const void *pos, const void *freq)
@@ -383,13 +424,21 @@ int norm_plan(NormArgs &a, int dtype, int b, bool bwd, long mask)
     for (Side &s : a.side) s.d = Div(s.heads > 0 ? s.heads : 1);
     a.dpairs = Div(a.pairs > 0 ? a.pairs : 1);
     a.dper = Div(a.per > 0 ? a.per : 1);
-    const int v = piece(dtype, a.D, a.pairs, mask);
+    // Narrow pieces waste the memory's width: where whole rows allow wider ones, the pairs are exchanged through LDS instead (fp16 8 x 2048 tokens, 20
+    // heads of 96, 17 pairs: forward 130 -> 65 us, with gradients 361 -> 165; heads of 128, 21 pairs: 123 -> 63, 369 -> 167).
+    int v = piece(dtype, a.D, a.pairs, mask);
+    const int whole = piece(dtype, a.D, 0, mask);
+    a.exchange = whole > v;
+    if (a.exchange) v = whole;
+    a.pitch = a.exchange ? a.pairs + a.pairs / 16 + 1 : a.pairs;
     a.units = pa_div_up(a.D, 2 * v);
     a.lpr = 1;
     while (a.lpr < a.units && a.lpr < 64) a.lpr <<= 1;
     a.tb = turn_tokens(a.tokens, a.side[0].heads + a.side[1].heads, a.lpr, bwd);
     return v;
 }
+
+size_t lds_of(const NormArgs &a) { return ((size_t)2 * a.tb * a.pitch + (a.exchange ? (256 / a.lpr) * (a.D + a.D / 16 + 1) : 0)) * 4; }
 
 }  // namespace
 
@@ -410,7 +459,7 @@ PA_API int pa_qk_norm_rotary(int dtype, int b, int n, int h, int hk, int d, cons
     const int v = norm_plan(a, dtype, b, false, alignment_of(es, {q, k, q_out, k_out}, {qb, qn, qh, kb, kn, kh, d}));
     const long groups = (a.tokens + a.tb - 1) / a.tb;
     PA_REQUIRE(groups < (1l << 31), "pa_qk_norm_rotary: too many workgroups");
-    const size_t lds = (size_t)2 * a.tb * a.pairs * 4;
+    const size_t lds = lds_of(a);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == F32) launch_norm<float, false>(a, v, dim3((unsigned)groups), lds, st);
     else if (dtype == F16) launch_norm<_Float16, false>(a, v, dim3((unsigned)groups), lds, st);
@@ -439,7 +488,7 @@ PA_API int pa_qk_norm_rotary_backward(int dtype, int b, int n, int h, int hk, in
     const int es = dtype == F32 ? 4 : 2;
     const int v = norm_plan(a, dtype, b, true, alignment_of(es, {q, k, gq, gk, dq, dk}, {qb, qn, qh, kb, kn, kh, gqb, gqn, gqh, gkb, gkn, gkh, d}));
     const int groups = groups_of(a.tokens, a.tb);
-    size_t lds = (size_t)2 * a.tb * a.pairs * 4;
+    size_t lds = lds_of(a);
     if (lds < (size_t)2 * d * 4) lds = (size_t)2 * d * 4;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == F32) launch_norm<float, true>(a, v, dim3(groups), lds, st);

@@ -3,7 +3,7 @@
 //     o_i = sum_j P_ij v_j,   P_ij = exp(s_ij) / sum_j exp(s_ij),   s_ij = scale q_i . k_j   over the keys j in view of row i (View, pa_attn.h)
 //
 // One pass over the keys with a running maximum and sum: O(window) work and nothing N x M in memory.  A workgroup owns 128 (float32: 64) rows -- the N
-// queries of the G heads that share a key head, query-major, so that one tile of keys serves all of them -- and walks the 64-key tiles that its rows can
+// queries of the G heads that share a key head, query-major, so that one tile of keys serves all of them -- and walks the tiles of 64 (32) keys that its rows can
 // see: the tiles of the first tokens, then one contiguous range.  A wave owns 32 rows.  S^T = K Q^T puts one row into a lane's registers (maximum and
 // sum need one exchange between the two half waves), and the registers of P^T feed O^T += V^T P^T without leaving the lane; V is read transposed
 // from LDS.  Tiles go straight from memory into the other half of a double buffer while the present one is used, one barrier a tile.
@@ -16,8 +16,8 @@
 // 64: 91 us = 755.  A 32 x 32 part costs 512 cycles of MFMA (width 128), about 600 of vector instructions (256 of them the 16 exponentials) and 512 of the
 // CU's LDS reads, on pipes that overlap only between the two to four waves of a SIMD: that is the bound.  Reading ahead by one product within a
 // wave (scores of the next part beside the exponentials of this one) cost more in registers than it hid (80 against 65 us at width 64).
-// float32 18 x 1024, 8 heads of 32, 128 keys either side: 88 us = 52 of the 153 TFLOP/s of a library product: MFMA at 2048 cycles a part, 1.5
-// rounds of workgroups, a quarter of the keys in the parts out of view.
+// float32 72 x 1024, 8 heads of 64, all keys: 1245 us = 124 of the 153 TFLOP/s of a library product; 18 x 1024, 8 heads of 32, 128 keys either side: 76 us =
+// 60: a quarter of the keys in its parts are out of view, and it is nine waves per SIMD in all, whose start and end nothing covers.
 #include "pa_attn.h"
 
 using namespace pa_attn;
