@@ -146,28 +146,28 @@ def _floats(n, device):
 
 
 # ------------------------------------------------------------------------------------------------------------------ norm and rotation
-def _norm_args(dt, q, k, qw, kw, pos, freq, eps, interleaved):
+def _norm_args(q, k, qw, kw, pos, freq, rest):
+    """rest: axes, frequencies of an axis, elements between two sequences' positions, eps, interleaved."""
     B, N, H, D = q.shape
     w = qw if qw is not None else kw
-    axes, per = freq.shape if freq is not None else (0, 0)
-    head = (dt, B, N, H, k.shape[2], D, ptr(q), *_strides(q), ptr(k), *_strides(k), ptr(qw), ptr(kw), int(w is not None and w.dtype == torch.float32))
-    place = (ptr(pos), _PTYPE[pos.dtype] if pos is not None else 0, N * axes if pos is not None and pos.dim() == 3 else 0, ptr(freq), axes, per)
-    return head + place + (eps, interleaved)
+    axes, per, apart, eps, interleaved = rest
+    return (_DTYPE[q.dtype], B, N, H, k.shape[2], D, ptr(q), *_strides(q), ptr(k), *_strides(k), ptr(qw), ptr(kw), int(w is not None and w.dtype == torch.float32),
+            ptr(pos), _PTYPE[pos.dtype] if axes else 0, apart, ptr(freq), axes, per, eps, interleaved)
 
 
-def _norm_forward(q, k, qw, kw, pos, freq, eps, interleaved):
+def _norm_forward(q, k, qw, kw, pos, freq, rest):
     out = q.new_empty(q.shape), k.new_empty(k.shape)
     with _on(q.device):
-        call("pa_qk_norm_rotary", *_norm_args(_DTYPE[q.dtype], q, k, qw, kw, pos, freq, eps, interleaved), ptr(out[0]), ptr(out[1]))
+        call("pa_qk_norm_rotary", *_norm_args(q, k, qw, kw, pos, freq, rest), ptr(out[0]), ptr(out[1]))
     return out
 
 
 class _NormRotary(Function):
     @staticmethod
-    def forward(ctx, q, k, qw, kw, pos, freq, eps, interleaved):
-        out = _norm_forward(q, k, qw, kw, pos, freq, eps, interleaved)
+    def forward(ctx, q, k, qw, kw, pos, freq, rest):
+        out = _norm_forward(q, k, qw, kw, pos, freq, rest)
         ctx.save_for_backward(q, k, qw, kw, pos, freq)
-        ctx.rest = eps, interleaved
+        ctx.rest = rest
         return out
 
     @staticmethod
@@ -185,10 +185,10 @@ class _NormRotary(Function):
             scratch = None
             if dqw is not None or dkw is not None:
                 scratch = _floats(_size("pa_qk_norm_rotary_backward_scratch_floats", q.shape[0], q.shape[1], D), q.device)
-            call("pa_qk_norm_rotary_backward", *_norm_args(_DTYPE[q.dtype], q, k, qw, kw, pos, freq, *ctx.rest), ptr(gq), *_strides(gq), ptr(gk), *_strides(gk),
+            call("pa_qk_norm_rotary_backward", *_norm_args(q, k, qw, kw, pos, freq, ctx.rest), ptr(gq), *_strides(gq), ptr(gk), *_strides(gk),
                  ptr(dq), ptr(dk), ptr(dqw), ptr(dkw), ptr(scratch))
         cast = [None if g is None else g.to(w.dtype) for g, w in ((dqw, qw), (dkw, kw))]
-        return dq, dk, cast[0], cast[1], None, None, None, None
+        return dq, dk, cast[0], cast[1], None, None, None
 
 
 def qk_norm_rotary(q, k, q_weight=None, k_weight=None, *, positions=None, inv_freq=None, eps=1e-6, interleaved=False):
@@ -210,35 +210,35 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, *, positions=None, inv_fr
         raise ValueError(f"{name}: head width {D} is not in 1..512, or no heads ({H}, {k.shape[2]})")
     ws = [w for w in (q_weight, k_weight) if w is not None]
     for w in ws:
-        if w.device != q.device or w.dtype not in (torch.float32, q.dtype) or tuple(w.shape) != (D,) or w.dtype != ws[0].dtype:
+        if w.get_device() != q.get_device() or w.dtype not in (torch.float32, q.dtype) or w.dim() != 1 or w.shape[0] != D or w.dtype != ws[0].dtype:
             raise ValueError(f"{name}: weights have to be ({D},) on {q.device}, both float32 or both {q.dtype}")
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"{name}: eps has to be finite and not negative")
     if (positions is None) != (inv_freq is None):
         raise ValueError(f"{name}: positions and inv_freq come together")
+    A, F, apart = 0, 0, 0
     if positions is not None:
-        if inv_freq.dtype != torch.float32 or inv_freq.device != q.device or inv_freq.dim() not in (1, 2) or inv_freq.numel() == 0:
+        if inv_freq.dtype != torch.float32 or inv_freq.get_device() != q.get_device() or inv_freq.dim() not in (1, 2) or inv_freq.numel() == 0:
             raise ValueError(f"{name}: inv_freq has to be a float32 (F,) or (A, F) tensor on {q.device}")
-        if positions.dtype not in _PTYPE or positions.device != q.device:
+        if positions.dtype not in _PTYPE or positions.get_device() != q.get_device():
             raise TypeError(f"{name}: positions have to be int32, int64 or float32 on {q.device}")
         if positions.requires_grad or inv_freq.requires_grad:
             raise RuntimeError(f"{name}: positions and inv_freq have no gradient here")
-        if inv_freq.dim() == 1:
-            inv_freq = inv_freq.view(1, -1)
-        A = inv_freq.shape[0]
-        if 2 * inv_freq.numel() > D:
-            raise ValueError(f"{name}: {A} x {inv_freq.shape[1]} frequencies rotate more than the {D} elements of a head")
+        A, F = inv_freq.shape if inv_freq.dim() == 2 else (1, inv_freq.shape[0])
+        if 2 * A * F > D:
+            raise ValueError(f"{name}: {A} x {F} frequencies rotate more than the {D} elements of a head")
         shape = tuple(positions.shape)
-        if A == 1 and shape in ((N,), (B, N)):
-            positions = positions.unsqueeze(-1)
-        elif shape not in ((N, A), (B, N, A)):
+        if shape == (B, N, A) or (A == 1 and shape == (B, N)):
+            apart = N * A
+        elif shape != (N, A) and not (A == 1 and shape == (N,)):
             raise ValueError(f"{name}: positions of shape {shape} fit neither (N, A) = ({N}, {A}) nor (B, N, A) with B = {B}")
         positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    rest = A, F, apart, float(eps), int(bool(interleaved))
     q, k = _unit(q), _unit(k)
     qw, kw = (w.contiguous() if w is not None else None for w in (q_weight, k_weight))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any(w.requires_grad for w in ws)):
-        return _NormRotary.apply(q, k, qw, kw, positions, inv_freq, float(eps), int(bool(interleaved)))
-    return _norm_forward(q, k, qw, kw, positions, inv_freq, float(eps), int(bool(interleaved)))
+        return _NormRotary.apply(q, k, qw, kw, positions, inv_freq, rest)
+    return _norm_forward(q, k, qw, kw, positions, inv_freq, rest)
 
 
 # ------------------------------------------------------------------------------------------------------------------- window attention

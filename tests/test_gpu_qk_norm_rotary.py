@@ -257,3 +257,24 @@ def test_refusals():
             (lambda: qk_norm_rotary(torch.zeros(1, 1, 1, 513, device="cuda"), torch.zeros(1, 1, 1, 513, device="cuda")), ValueError)]:
         with pytest.raises(exc):
             bad()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D,P", [(16, 1), (16, 3), (32, 15), (48, 21), (64, 31), (96, 17), (128, 21), (128, 63), (192, 95), (256, 5), (512, 255), (66, 32), (132, 33)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_pair_counts_that_leave_half_a_piece(dtype, D, P, inter):
+    """Pairs whose second halves, or whose rest, do not start at a whole piece: exchanged between lanes.  More rows than one turn holds."""
+    pos = torch.arange(150, device="cuda", dtype=torch.int32)
+    _check(1, 150, 3, 1, D, dtype, freq=_freq(1, P), pos=pos, inter=inter, seed=D + P)
+
+
+def test_positions_of_one_token():
+    """(N,), (B, N), (N, 1) and (B, N, 1) name the same positions where they can be mistaken for each other."""
+    from patchaugnet_amd.attention import qk_norm_rotary
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k = (torch.randn(2, 1, 2, 16, generator=g, device="cuda") for _ in range(2))
+    fr = _freq(1, 8)
+    want = qk_norm_rotary(q, k, positions=torch.tensor([[5], [5]], device="cuda"), inv_freq=fr)
+    for pos in (torch.tensor([5], device="cuda"), torch.tensor([[5]], device="cuda"), torch.tensor([[[5]], [[5]]], device="cuda")):
+        got = qk_norm_rotary(q, k, positions=pos, inv_freq=fr.view(-1) if pos.dim() == 1 else fr)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
