@@ -52,6 +52,8 @@ __device__ __forceinline__ void mma(pa_f16v &c, const pa_f8 &a, const pa_f8 &b)
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
 }
 
+// the larger of two scores, NaN if one is: v_maximum3_f32 takes three without the canonicalising moves that fmaxf needs on a product's registers
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // value of the lane with the other l / 32

@@ -105,8 +105,8 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
             }
             float mt = s[0];
 #pragma unroll
-            for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
-            mt = fmaxf(mt, other_half(mt)) * a.c;
+            for (int r = 1; r < 16; ++r) mt = larger(mt, s[r]);
+            mt = larger(mt, other_half(mt)) * a.c;
             if (__any(mt > m_run + 8.f)) {                     // -inf + 8 = -inf: the first visible key of a row always moves it
                 const float mn = fmaxf(m_run, mt), sc = mn > -INFINITY ? ex2(m_run - mn) : 0.f;
 #pragma unroll
