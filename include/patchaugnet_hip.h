@@ -529,15 +529,15 @@ int pa_qk_norm_rotary_backward(int dtype, int b, int n, int h, int hk, int d, co
                                float *dqw, float *dkw, float *scratch, pa_stream_t stream);
 
 /* out (b,n,h,d, contiguous) = softmax(scale q k^T over the keys in view) v; q (b,n,h,d), k and v (b,m,hk,d), d a multiple of 8 up to 128.
- * kn, vn (backward: qn, qh, gn, gh too) <= 2^22.  lse (b,h,n; NULL: not wanted): log2 of the sum of exponentials, for the backward pass.  scratch: as many floats as the function says (0: NULL). */
+ * kn, vn (backward: qn, qh, gn, gh too) <= 2^22.  low (as out; NULL: not wanted): out minus its rounding, and lse (b,h,n; NULL: not wanted): log2 of the sum of exponentials, for the backward pass.  scratch: as many floats as the function says (0: NULL). */
 long pa_window_attention_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks);
 int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn, long kh,
                         const void *v, long vb, long vn, long vh, int left, int right, int sinks, float scale, const int *start, const int *length, void *out,
-                        float *lse, float *scratch, pa_stream_t stream);
-/* dq, dk, dv (contiguous) from dout (b,n,h,d) and the forward's out and lse.  Sums in a fixed order: the same bits every time. */
+                        void *low, float *lse, float *scratch, pa_stream_t stream);
+/* dq, dk, dv (contiguous) from dout (b,n,h,d) and the forward's out, low (NULL: taken as 0) and lse.  Sums in a fixed order: the same bits every time. */
 long pa_window_attention_backward_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks);
 int pa_window_attention_backward(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn,
-                                 long kh, const void *v, long vb, long vn, long vh, const void *out, const float *lse, const void *dout, long gb, long gn, long gh,
+                                 long kh, const void *v, long vb, long vn, long vh, const void *out, const void *low, const float *lse, const void *dout, long gb, long gn, long gh,
                                  int left, int right, int sinks, float scale, const int *start, const int *length, void *dq, void *dk, void *dv, float *scratch,
                                  pa_stream_t stream);
 

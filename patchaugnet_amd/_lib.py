@@ -118,8 +118,8 @@ _SIGS = {
     "pa_fp_chain_premul_g16h": "ipppplppppiiiippp",
     "pa_qk_norm_rotary": "iiiiii" + "plll" * 2 + "ppipilpiifipp",
     "pa_qk_norm_rotary_backward": "iiiiii" + "plll" * 2 + "ppipilpiifi" + "plll" * 2 + "ppppp",
-    "pa_window_attention": "iiiiiii" + "plll" * 3 + "iiifppppp",
-    "pa_window_attention_backward": "iiiiiii" + "plll" * 3 + "pp" + "plll" + "iiifpppppp",
+    "pa_window_attention": "iiiiiii" + "plll" * 3 + "iiifpppppp",
+    "pa_window_attention_backward": "iiiiiii" + "plll" * 3 + "ppp" + "plll" + "iiifpppppp",
     "pa_paged_attention": "iiiii" + "pll" + "plll" * 2 + "iipipiifpp",
     "pa_paged_append": "iiiii" + "plll" * 4 + "iipipp",
 }

@@ -246,30 +246,31 @@ def _window_sizes(q, k, view):
     return q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], view[0], view[1], view[2]
 
 
-def _window_forward(q, k, v, start, length, view, want_lse):
+def _window_forward(q, k, v, start, length, view, back):
     out = q.new_empty(q.shape)
+    low = q.new_empty(q.shape) if back and q.dtype != torch.float32 else None
     B, N, H, D = q.shape
-    lse = torch.empty((B, H, N), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty((B, H, N), dtype=torch.float32, device=q.device) if back else None
     left, right, sinks, scale = view
     with _on(q.device):
         scratch = _floats(_size("pa_window_attention_scratch_floats", *_window_sizes(q, k, view)), q.device)
         call("pa_window_attention", _DTYPE[q.dtype], B, N, k.shape[1], H, k.shape[2], D, ptr(q), *_strides(q), ptr(k), *_strides(k), ptr(v), *_strides(v),
-             left, right, sinks, scale, ptr(start), ptr(length), ptr(out), ptr(lse), ptr(scratch))
-    return out, lse
+             left, right, sinks, scale, ptr(start), ptr(length), ptr(out), ptr(low), ptr(lse), ptr(scratch))
+    return out, low, lse
 
 
 class _WindowAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, start, length, view):
-        out, lse = _window_forward(q, k, v, start, length, view, True)
-        ctx.save_for_backward(q, k, v, start, length, out, lse)
+        out, low, lse = _window_forward(q, k, v, start, length, view, True)
+        ctx.save_for_backward(q, k, v, start, length, out, low, lse)
         ctx.view = view
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q, k, v, start, length, out, lse = ctx.saved_tensors
+        q, k, v, start, length, out, low, lse = ctx.saved_tensors
         g = _rows(g, far=_FAR)
         left, right, sinks, scale = ctx.view
         dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
@@ -277,7 +278,7 @@ class _WindowAttention(Function):
         with _on(q.device):
             scratch = _floats(_size("pa_window_attention_backward_scratch_floats", *_window_sizes(q, k, ctx.view)), q.device)
             call("pa_window_attention_backward", _DTYPE[q.dtype], B, N, k.shape[1], H, k.shape[2], D, ptr(q), *_strides(q), ptr(k), *_strides(k), ptr(v),
-                 *_strides(v), ptr(out), ptr(lse), ptr(g), *_strides(g), left, right, sinks, scale, ptr(start), ptr(length), ptr(dq), ptr(dk), ptr(dv),
+                 *_strides(v), ptr(out), ptr(low), ptr(lse), ptr(g), *_strides(g), left, right, sinks, scale, ptr(start), ptr(length), ptr(dq), ptr(dk), ptr(dv),
                  ptr(scratch))
         return dq, dk, dv, None, None, None
 

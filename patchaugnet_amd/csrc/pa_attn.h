@@ -187,6 +187,15 @@ template <typename T> __device__ __forceinline__ typename Frag<T>::type pack(con
     return f;
 }
 
+// what pack() rounded away, as a fragment of its own: with it a product takes the registers to twice the type's digits
+template <typename T> __device__ __forceinline__ typename Frag<T>::type pack_rest(const pa_f16v &a, const typename Frag<T>::type &f, int u)
+{
+    typename Frag<T>::type g;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = (T)(a[8 * u + e] - (float)f[e]);
+    return g;
+}
+
 // fragment of a row held in global memory: elements 16 kk + 8 h .. of `row`, zeros past d (a multiple of 8)
 template <typename T> __device__ __forceinline__ typename Frag<T>::type ldrow(const T *row, int kk, int h, int d, bool ok)
 {
@@ -271,6 +280,12 @@ template <int KT> struct TileList {
 // 512: 62 / 83; 16384 tokens of 128, window 1024: 748 / 832; float32 4 x 2048 x 8 of 64 and 128, window 256: 64 / 60 and 142 / 127; dk and dv of the
 // latter 209 / 184 and 454 / 447, of fp16 8 x 4096 x 8 of 96 with 64 keys either side 122 / 103, of bf16 4 x 2048 x 16 of 64, all keys: 193 / 236.
 static inline int waves_of(int es, long reach) { return es == 4 || reach < 256 ? 2 : 4; }
+
+// 16-bit training passes over few (query, key) pairs multiply weights and dS as the sum of their rounding and the rest's.  Rounded once, dS adds as much to
+// the error of dq and dk as their own rounding does (1.41 times it together) where many pairs average out; up to 1.53 times it was seen below 2^22
+// pairs, and 1.97 for sequences of two or three tokens.  The second part costs 1.0 and 1.6 us (dq 8.0, dk and dv 9.8) at 2^20 pairs, 32 wide, 1.5 and 2.3 us
+// of 13 at 2^22, 64 wide; at 2^24 it would be 2.9 of 20.7 and 4.7 of 31.4, where it gains nothing.
+static inline bool few_pairs(long heads, long n, long m, long reach) { return heads * n * (m < reach ? m : reach) <= (1l << 22); }
 
 // waves on a SIMD that the registers are held down to
 template <typename T, int DT> constexpr int waves_per_simd() { return sizeof(T) == 2 ? 2 : DT <= 32 ? 3 : DT <= 64 ? 2 : 1; }

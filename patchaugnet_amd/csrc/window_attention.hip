@@ -9,7 +9,11 @@
 // from LDS.  Tiles go straight from memory into the other half of a double buffer while the present one is used, one barrier a tile.
 //
 // Roundings: s, maximum, sum and o are 32-bit; P is rounded to the type of V for the second product (16-bit types), with P <= 2^8 by the running
-// maximum, which is only moved when a row's maximum grows by more than 2^8 (the quotient is the same for any reference value).
+// maximum, which is only moved when a row's maximum grows by more than 2^8 (the quotient is the same for any reference value).  Where a backward pass
+// follows, its delta is a difference that magnifies the error of o: what the rounding of o leaves is handed on beside it, and for heads of 8 and 16 (where
+// dq was off by 1.50 to 1.52 times the rounding of the result, now 1.47; wider ones by 1.48 at most) and few pairs (few_pairs()) P is multiplied as the
+// sum of its rounding and the rest's -- without gradients too, so that out has the same bits with and without.  4 x 4096 tokens, 16 heads over 4 in a tile
+// 32 wide, window 512: 45 us, in two parts 60.
 //
 // Measured: bf16 4 x 16384 tokens, 16 heads of 128 over 4, window 1024: 660 us = 810 TFLOP/s of visible pairs (a library product of that type: 1219;
 // 12 % of the work is keys of tiles that a row does not see); 4 x 4096, 16 heads of 64 over 4, window 512: 60 us = 540; all keys of 4 x 2048, 16 heads of
@@ -26,16 +30,25 @@ namespace {
 
 struct FwdArgs {
     const void *q, *k, *v;
-    void *out;
+    void *out, *low;
     float *lse, *part;
     long qb, qn, qh, kb, kn, kh, vb, vn, vh;
     int B, N, H, Hk, D, G, splits, nqt;
+    bool few;
     float c;                  // scale log2(e)
     View view;
     Div g;
 };
 
-template <typename T, int DT, int NW, bool SPLIT>
+// four elements of the output and, for the backward pass, what their rounding left
+template <typename T> __device__ __forceinline__ void store_out(T *out, T *low, pa_f4 x)
+{
+    st4<T>(out, x[0], x[1], x[2], x[3]);
+    if (low) st4<T>(low, x[0] - (float)(T)x[0], x[1] - (float)(T)x[1], x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
+}
+
+// FINE: the product with V takes P in two parts
+template <typename T, int DT, int NW, bool SPLIT, bool FINE>
 __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel(const FwdArgs a)
 {
     typedef Tile<T, DT> L;
@@ -125,8 +138,14 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const F p = pack<T>(s, u);
+                F rest;
+                if constexpr (FINE) rest = pack_rest<T>(s, p, u);
 #pragma unroll
-                for (int ct = 0; ct < DT / 32; ++ct) mma(o[ct], L::ldt(vs, sub * 32 + 16 * u, ct * 32), p);
+                for (int ct = 0; ct < DT / 32; ++ct) {
+                    const F v = L::ldt(vs, sub * 32 + 16 * u, ct * 32);
+                    mma(o[ct], v, p);
+                    if constexpr (FINE) mma(o[ct], v, rest);
+                }
             }
         }
     };
@@ -152,13 +171,14 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
         return;
     }
     const float inv = keys.ok && l_run != 0.f ? 1.0f / l_run : 0.f;         // padding rows computed on zeros: their output is 0
-    T *op = (T *)a.out + (((size_t)b * a.N + i) * a.H + hq) * a.D;
+    const size_t place = (((size_t)b * a.N + i) * a.H + hq) * a.D;
+    T *op = (T *)a.out + place, *low = a.low ? (T *)a.low + place : nullptr;
 #pragma unroll
     for (int ct = 0; ct < DT / 32; ++ct)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int c = ct * 32 + 8 * u + 4 * h;
-            if (c < a.D) st4<T>(op + c, o[ct][4 * u] * inv, o[ct][4 * u + 1] * inv, o[ct][4 * u + 2] * inv, o[ct][4 * u + 3] * inv);
+            if (c < a.D) store_out<T>(op + c, low ? low + c : nullptr, (pa_f4){o[ct][4 * u] * inv, o[ct][4 * u + 1] * inv, o[ct][4 * u + 2] * inv, o[ct][4 * u + 3] * inv});
         }
     if (a.lse && h == 0) a.lse[((size_t)b * a.H + hq) * a.N + i] = inv == 0.f ? INFINITY : m_run + __builtin_amdgcn_logf(l_run);
 }
@@ -188,7 +208,8 @@ __global__ __launch_bounds__(256) void join_kernel(const FwdArgs a)
     const int bh = (int)(at / rows), row = (int)(at - (size_t)bh * rows), b = bh / a.Hk, hk = bh - b * a.Hk;
     const int i = a.g.div(row), hq = hk * a.G + row - i * a.G;
     const float inv = a.view.first(b) + i < a.view.len(b) && l != 0.f ? 1.0f / l : 0.f;
-    if (c < a.D) st4<T>((T *)a.out + (((size_t)b * a.N + i) * a.H + hq) * a.D + c, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    const size_t place = (((size_t)b * a.N + i) * a.H + hq) * a.D + c;
+    if (c < a.D) store_out<T>((T *)a.out + place, a.low ? (T *)a.low + place : nullptr, o * inv);
     if (a.lse && c == 0) a.lse[((size_t)b * a.H + hq) * a.N + i] = inv == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -215,22 +236,25 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int es, int left, int right, 
     return s;
 }
 
-template <typename T, int DT, int NW, bool SPLIT>
+template <typename T, int DT, int NW, bool SPLIT, bool FINE>
 void launch_rows(const FwdArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((fwd_kernel<T, DT, NW, SPLIT>), dim3((unsigned)((long)a.nqt * a.B * a.Hk), (unsigned)a.splits), dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL((fwd_kernel<T, DT, NW, SPLIT, FINE>), dim3((unsigned)((long)a.nqt * a.B * a.Hk), (unsigned)a.splits), dim3(64 * NW), 0, st, a);
 }
 
 template <typename T, int DT>
 int launch_fwd(const FwdArgs &a, hipStream_t st)
 {
     constexpr int NW = sizeof(T) == 4 ? 2 : 4;
+    const bool fine = a.few || a.D <= 16;
     if (a.splits > 1) {
-        launch_rows<T, DT, NW, true>(a, st);
+        if (fine) launch_rows<T, DT, NW, true, sizeof(T) == 2>(a, st);
+        else launch_rows<T, DT, NW, true, false>(a, st);
         const long threads = (long)a.B * a.Hk * a.N * a.G * (DT / 4);
         hipLaunchKernelGGL((join_kernel<T, DT>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
     } else {
-        launch_rows<T, DT, NW, false>(a, st);
+        if (fine) launch_rows<T, DT, NW, false, sizeof(T) == 2>(a, st);
+        else launch_rows<T, DT, NW, false, false>(a, st);
     }
     return 0;
 }
@@ -247,16 +271,16 @@ PA_API long pa_window_attention_scratch_floats(int b, int n, int m, int h, int h
 
 PA_API int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb, long kn,
                                long kh, const void *v, long vb, long vn, long vh, int left, int right, int sinks, float scale, const int *start,
-                               const int *length, void *out, float *lse, float *scratch, pa_stream_t stream)
+                               const int *length, void *out, void *low, float *lse, float *scratch, pa_stream_t stream)
 {
     int rc = window_attention_check("pa_window_attention", dtype, b, n, m, h, hk, d, left, right, sinks, scale);
     if (rc != PA_OK) return rc;
     if (b == 0 || n == 0) return PA_OK;
     PA_REQUIRE(q && out && (m == 0 || (k && v)), "pa_window_attention: null tensor");
-    PA_REQUIRE(alignment_of(dtype == PA_DT_F32 ? 4 : 2, {q, k, v, out}, {qb, qn, qh, kb, kn, kh, vb, vn, vh}) == 16,
+    PA_REQUIRE(alignment_of(dtype == PA_DT_F32 ? 4 : 2, {q, k, v, out, low}, {qb, qn, qh, kb, kn, kh, vb, vn, vh}) == 16,
                "pa_window_attention: addresses and strides have to be multiples of 16 bytes");
     FwdArgs a;
-    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.part = scratch;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.low = low; a.lse = lse; a.part = scratch;
     a.qb = qb; a.qn = qn; a.qh = qh; a.kb = kb; a.kn = kn; a.kh = kh; a.vb = vb; a.vn = vn; a.vh = vh;
     a.B = b; a.N = n; a.H = h; a.Hk = hk; a.D = d; a.G = h / hk;
     a.view.m = m; a.view.left = left < 0 ? UNBOUNDED : left; a.view.right = right < 0 ? UNBOUNDED : right; a.view.sinks = sinks < m ? sinks : m;
@@ -265,6 +289,7 @@ PA_API int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, in
     a.g = Div(a.G);
     const Shape sh = shape_of(b, n, m, h, hk, dtype == PA_DT_F32 ? 4 : 2, a.view.left, a.view.right, sinks);
     a.nqt = sh.nqt;
+    a.few = few_pairs((long)b * h, n, m, (long)a.view.left + a.view.right + 1);
     a.splits = sh.splits;
     PA_REQUIRE(kn >= 0 && vn >= 0 && kn <= PA_ATTN_MAXSTRIDE && vn <= PA_ATTN_MAXSTRIDE, "pa_window_attention: tokens are more than 2^22 elements apart");
     PA_REQUIRE((long)a.nqt * b * hk < (1l << 31), "pa_window_attention: too many workgroups");

@@ -12,8 +12,9 @@
 // workgroups of their own, 32 keys each: there the waves share the keys and take the rows in turn.  They write 32-bit partial sums, joined with the
 // window's by a second launch; all walks are cut into such slices when the keys alone do not fill the chip.
 //
-// Roundings: P and dS are rounded to the operand type for the second products (16-bit types); the scale is applied to the 32-bit sums, so that dS is
-// rounded before it gets smaller.
+// Roundings: P and dS are rounded to the operand type for the second products (16-bit types; the sum of two parts for few pairs, few_pairs()); the scale
+// is applied to the 32-bit sums, so that dS is rounded before it gets smaller.  delta takes o as the forward pass had it before it was rounded
+// (out + low): dP - delta is small beside delta, and with the rounded o alone dq and dk were off by 1.6 times the rounding of the result, now 1.42 to 1.47.
 //
 // Measured, dq / dk and dv / join: bf16 4 x 4096 tokens, 16 heads of 64 over 4, window 512: 77 / 113 / 5 us (630 / 575 TFLOP/s of visible pairs); all keys of
 // 4 x 2048, 16 heads of 64: 114 / 157 us (900 / 870; a library product: 1219); 2 x 8192, 16 of 128 over 4, window 1024: 215 / 466 / 7 us; float32
@@ -29,7 +30,7 @@ namespace {
 template <typename T, int DT> constexpr int row_tile() { return DT * (int)sizeof(T) >= 512 ? 32 : 64; }
 
 struct BwdArgs {
-    const void *q, *k, *v, *out, *dout;
+    const void *q, *k, *v, *out, *low, *dout;
     const float *lse;
     float *delta, *part;
     void *dq, *dk, *dv;
@@ -38,12 +39,14 @@ struct BwdArgs {
     int nkt, slices;                   // key tiles, slices of their walks
     int nst, groups, fars;             // key tiles with first tokens, groups of 32 first tokens that have far rows, slices of their walks
     int rt;                            // rows of a tile: as many whole queries as fit
+    bool few;
     float c, scale;
     View view;
     Div g;
 };
 
-template <typename T, int DT, int NW>
+// FINE: the second products take P and dS in two parts
+template <typename T, int DT, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(const BwdArgs a)
 {
     typedef Tile<T, DT> L;
@@ -63,15 +66,20 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
     float delta = 0.f;
     {
         const T *qp = (const T *)a.q + b * a.qb + i * a.qn + hq * a.qh, *gp = (const T *)a.dout + b * a.gb + i * a.gn + hq * a.gh;
-        const T *op = (const T *)a.out + (((size_t)b * a.N + i) * a.H + hq) * a.D;
+        const size_t place = (((size_t)b * a.N + i) * a.H + hq) * a.D;
+        const T *op = (const T *)a.out + place, *lp = a.low ? (const T *)a.low + place : op;
+        F of[DT / 16], lf[DT / 16];
 #pragma unroll
         for (int kk = 0; kk < DT / 16; ++kk) {
             qf[kk] = ldrow<T>(qp, kk, h, a.D, keys.ok);
             gf[kk] = ldrow<T>(gp, kk, h, a.D, keys.ok);
-            const F of = ldrow<T>(op, kk, h, a.D, keys.ok);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)gf[kk][e], (float)of[e], delta);
+            of[kk] = ldrow<T>(op, kk, h, a.D, keys.ok);
+            lf[kk] = ldrow<T>(lp, kk, h, a.D, keys.ok && a.low);
         }
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)gf[kk][e], (float)of[kk][e] + (float)lf[kk][e], delta);
         delta += other_half(delta);
     }
     const float lse = keys.ok ? a.lse[at] : INFINITY;
@@ -122,8 +130,14 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const F ds = pack<T>(s, u);
+                F rest;
+                if constexpr (FINE) rest = pack_rest<T>(s, ds, u);
 #pragma unroll
-                for (int ct = 0; ct < DT / 32; ++ct) mma(dq[ct], L::ldt(ks, sub * 32 + 16 * u, ct * 32), ds);
+                for (int ct = 0; ct < DT / 32; ++ct) {
+                    const F kt = L::ldt(ks, sub * 32 + 16 * u, ct * 32);
+                    mma(dq[ct], kt, ds);
+                    if constexpr (FINE) mma(dq[ct], kt, rest);
+                }
             }
         }
     };
@@ -177,7 +191,7 @@ struct Walk {
     }
 };
 
-template <typename T, int DT, int NW>
+template <typename T, int DT, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void dkv_kernel(const BwdArgs a)
 {
     typedef Tile<T, DT> L;
@@ -306,10 +320,20 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const F pf = pack<T>(s, u), df = pack<T>(dp, u);
+                F pr, dr;
+                if constexpr (FINE) {
+                    pr = pack_rest<T>(s, pf, u);
+                    dr = pack_rest<T>(dp, df, u);
+                }
 #pragma unroll
                 for (int ct = 0; ct < DT / 32; ++ct) {
-                    mma(dv[ct], L::ldt(gs, sub * 32 + 16 * u, ct * 32), pf);
-                    mma(dk[ct], L::ldt(qs, sub * 32 + 16 * u, ct * 32), df);
+                    const F gt = L::ldt(gs, sub * 32 + 16 * u, ct * 32), qt = L::ldt(qs, sub * 32 + 16 * u, ct * 32);
+                    mma(dv[ct], gt, pf);
+                    mma(dk[ct], qt, df);
+                    if constexpr (FINE) {
+                        mma(dv[ct], gt, pr);
+                        mma(dk[ct], qt, dr);
+                    }
                 }
             }
         }
@@ -392,8 +416,7 @@ struct Shape {
 };
 
 // Slices: keys that do not fill the chip (fewer than 2048 waves, two per SIMD) have their walks cut, each slice with at least four row tiles;
-// far rows are cut into slices of
-// 16 row tiles, more where the slices alone would fill the chip several times (2048 of them).
+// far rows are cut into slices of 16 row tiles, more where the slices alone would fill the chip several times (2048 of them).
 Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int right, int sinks, bool started)
 {
     Shape s;
@@ -419,28 +442,37 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int 
     return s;
 }
 
-template <typename T, int DT, int NW>
+template <typename T, int DT, int NW, bool FINE>
 void launch_dq(const BwdArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((dq_kernel<T, DT, NW>), dim3((unsigned)((long)a.nqt * a.B * a.Hk)), dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL((dq_kernel<T, DT, NW, FINE>), dim3((unsigned)((long)a.nqt * a.B * a.Hk)), dim3(64 * NW), 0, st, a);
 }
 
-template <typename T, int DT, int NW>
+template <typename T, int DT, int NW, bool FINE>
 void launch_dkv(const BwdArgs &a, int joined, hipStream_t st)
 {
     const long bh = (long)a.B * a.Hk;
-    hipLaunchKernelGGL((dkv_kernel<T, DT, NW>), dim3((unsigned)(bh * a.groups * a.fars + bh * a.nkt * a.slices)), dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL((dkv_kernel<T, DT, NW, FINE>), dim3((unsigned)(bh * a.groups * a.fars + bh * a.nkt * a.slices)), dim3(64 * NW), 0, st, a);
     if (joined) hipLaunchKernelGGL((dkv_join_kernel<T, DT, NW>), dim3((unsigned)(bh * joined * 32 * NW)), dim3(256), 0, st, a, joined);
 }
 
 template <typename T, int DT>
 int launch_bwd(const BwdArgs &a, const Shape &s, hipStream_t st)
 {
-    if (a.nqt) launch_dq<T, DT, sizeof(T) == 4 ? 2 : 4>(a, st);
-    if (a.nkt) {
-        if constexpr (sizeof(T) == 4) launch_dkv<T, DT, 2>(a, s.joined(), st);
-        else if (s.kwaves == 2) launch_dkv<T, DT, 2>(a, s.joined(), st);
-        else launch_dkv<T, DT, 4>(a, s.joined(), st);
+    if constexpr (sizeof(T) == 4) {
+        if (a.nqt) launch_dq<T, DT, 2, false>(a, st);
+        if (a.nkt) launch_dkv<T, DT, 2, false>(a, s.joined(), st);
+    } else {
+        if (a.nqt) {
+            if (a.few) launch_dq<T, DT, 4, true>(a, st);
+            else launch_dq<T, DT, 4, false>(a, st);
+        }
+        if (a.nkt) {
+            if (s.kwaves == 2 && a.few) launch_dkv<T, DT, 2, true>(a, s.joined(), st);
+            else if (s.kwaves == 2) launch_dkv<T, DT, 2, false>(a, s.joined(), st);
+            else if (a.few) launch_dkv<T, DT, 4, true>(a, s.joined(), st);
+            else launch_dkv<T, DT, 4, false>(a, s.joined(), st);
+        }
     }
     return 0;
 }
@@ -461,7 +493,7 @@ PA_API long pa_window_attention_backward_scratch_floats(int b, int n, int m, int
 }
 
 PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb,
-                                        long kn, long kh, const void *v, long vb, long vn, long vh, const void *out, const float *lse, const void *dout, long gb,
+                                        long kn, long kh, const void *v, long vb, long vn, long vh, const void *out, const void *low, const float *lse, const void *dout, long gb,
                                         long gn, long gh, int left, int right, int sinks, float scale, const int *start, const int *length, void *dq, void *dk,
                                         void *dv, float *scratch, pa_stream_t stream)
 {
@@ -469,10 +501,10 @@ PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, i
     if (rc != PA_OK) return rc;
     if (b == 0 || (n == 0 && m == 0)) return PA_OK;
     PA_REQUIRE((n == 0 || (q && out && lse && dout && dq && scratch)) && (m == 0 || (k && v && dk && dv)), "pa_window_attention_backward: null tensor");
-    PA_REQUIRE(alignment_of(dtype == PA_DT_F32 ? 4 : 2, {q, k, v, out, dout, dq, dk, dv, scratch}, {qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh}) == 16,
+    PA_REQUIRE(alignment_of(dtype == PA_DT_F32 ? 4 : 2, {q, k, v, out, low, dout, dq, dk, dv, scratch}, {qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh}) == 16,
                "pa_window_attention_backward: addresses and strides have to be multiples of 16 bytes");
     BwdArgs a;
-    a.q = q; a.k = k; a.v = v; a.out = out; a.dout = dout; a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.low = low; a.dout = dout; a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv;
     a.delta = scratch;
     a.part = scratch + pa_div_up((long)b * h * n, 4) * 4l;
     a.qb = qb; a.qn = qn; a.qh = qh; a.kb = kb; a.kn = kn; a.kh = kh; a.vb = vb; a.vn = vn; a.vh = vh; a.gb = gb; a.gn = gn; a.gh = gh;
@@ -483,6 +515,7 @@ PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, i
     a.c = scale * 1.4426950408889634f;
     a.g = Div(a.G);
     const Shape s = shape_of(b, n, m, h, hk, d, dtype == PA_DT_F32 ? 4 : 2, a.view.left, a.view.right, sinks, start != nullptr);
+    a.few = few_pairs((long)b * h, n, m, (long)a.view.left + a.view.right + 1);
     a.nqt = s.nqt; a.nkt = s.nkt; a.slices = s.slices; a.nst = s.nst; a.groups = s.groups; a.fars = s.fars; a.rt = s.rt;
     PA_REQUIRE(kn >= 0 && vn >= 0 && kn <= PA_ATTN_MAXSTRIDE && vn <= PA_ATTN_MAXSTRIDE && qn >= 0 && qh >= 0 && gn >= 0 && gh >= 0 && qn <= PA_ATTN_MAXSTRIDE &&
                    gn <= PA_ATTN_MAXSTRIDE && qh <= PA_ATTN_MAXSTRIDE && gh <= PA_ATTN_MAXSTRIDE,

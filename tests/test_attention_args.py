@@ -29,8 +29,8 @@ def test_host_tensors_are_refused():
 def _window(lib, dtype=0, b=1, n=4, m=4, h=2, hk=1, d=32, left=-1, right=0, sinks=0, scale=1.0, back=False):
     p, z = ctypes.c_void_p(0), (ctypes.c_void_p(0), 0, 0, 0)
     if back:
-        return lib.pa_window_attention_backward(dtype, b, n, m, h, hk, d, *z, *z, *z, p, p, *z, left, right, sinks, scale, p, p, p, p, p, p, p)
-    return lib.pa_window_attention(dtype, b, n, m, h, hk, d, *z, *z, *z, left, right, sinks, scale, p, p, p, p, p, p)
+        return lib.pa_window_attention_backward(dtype, b, n, m, h, hk, d, *z, *z, *z, p, p, p, *z, left, right, sinks, scale, p, p, p, p, p, p, p)
+    return lib.pa_window_attention(dtype, b, n, m, h, hk, d, *z, *z, *z, left, right, sinks, scale, p, p, p, p, p, p, p)
 
 
 @pytest.mark.parametrize("back", [False, True])
@@ -97,9 +97,9 @@ def test_misaligned_addresses_are_refused(lib):
     at, off = ctypes.c_void_p(base), (ctypes.c_void_p(base + 8), 0, 32, 32)
     skew = (ctypes.c_void_p(base), 0, 34, 32)
     for bad in (off, skew):
-        assert lib.pa_window_attention(0, 1, 1, 1, 1, 1, 32, *bad, *z, *z, -1, 0, 0, 1.0, p, p, at, p, at, p) == -1
+        assert lib.pa_window_attention(0, 1, 1, 1, 1, 1, 32, *bad, *z, *z, -1, 0, 0, 1.0, p, p, at, p, p, at, p) == -1
         assert b"16 bytes" in lib.pa_last_error()
-        assert lib.pa_window_attention_backward(0, 1, 1, 1, 1, 1, 32, *z, *bad, *z, at, at, *z, -1, 0, 0, 1.0, p, p, at, at, at, at, p) == -1
+        assert lib.pa_window_attention_backward(0, 1, 1, 1, 1, 1, 32, *z, *bad, *z, at, p, at, *z, -1, 0, 0, 1.0, p, p, at, at, at, at, p) == -1
         assert lib.pa_paged_attention(0, 1, 1, 1, 32, at, 0, 32, *bad, *z, 1, 1, at, 1, at, -1, 0, 1.0, at, at, p) == -1
         assert lib.pa_paged_append(0, 1, 1, 1, 32, *bad, *z, *z, *z, 1, 1, at, 1, at, p, p) == -1
         assert b"16 bytes" in lib.pa_last_error()
