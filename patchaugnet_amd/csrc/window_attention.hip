@@ -15,11 +15,12 @@
 // sum of its rounding and the rest's -- without gradients too, so that out has the same bits with and without.  4 x 4096 tokens, 16 heads over 4 in a tile
 // 32 wide, window 512: 45 us, in two parts 60.
 //
-// Measured: bf16 4 x 16384 tokens, 16 heads of 128 over 4, window 1024: 660 us = 810 TFLOP/s of visible pairs (a library product of that type: 1219;
-// 12 % of the work is keys of tiles that a row does not see); 4 x 4096, 16 heads of 64 over 4, window 512: 60 us = 540; all keys of 4 x 2048, 16 heads of
-// 64: 91 us = 755.  A 32 x 32 part costs 512 cycles of MFMA (width 128), about 600 of vector instructions (256 of them the 16 exponentials) and 512 of the
-// CU's LDS reads, on pipes that overlap only between the two to four waves of a SIMD: that is the bound.  Reading ahead by one product within a
-// wave (scores of the next part beside the exponentials of this one) cost more in registers than it hid (80 against 65 us at width 64).
+// Measured: bf16 4 x 16384 tokens, 16 heads of 128 over 4, window 1024: 688 us = 780 TFLOP/s of visible pairs (a library product of that type: 1219;
+// 12 % of the work is keys of tiles that a row does not see); 4 x 4096, 16 heads of 64 over 4, window 512: 60 us = 540 (68 with what the rounding of out
+// leaves, for a backward pass); all keys of 4 x 2048, 16 heads of 64: 91 us = 755.  A 32 x 32 part costs 512 cycles of MFMA (width 128), about 600 of
+// vector instructions (256 of them the 16 exponentials) and 512 of the CU's LDS reads, on pipes that overlap only between the two to four waves of a
+// SIMD: that is the bound.  Reading ahead by one product within a wave (scores of the next part beside the exponentials of this one) cost more in
+// registers than it hid (80 against 65 us at width 64).
 // float32 72 x 1024, 8 heads of 64, all keys: 1245 us = 124 of the 153 TFLOP/s of a library product; 18 x 1024, 8 heads of 32, 128 keys either side: 76 us =
 // 60: a quarter of the keys in its parts are out of view, and it is nine waves per SIMD in all, whose start and end nothing covers.
 #include "pa_attn.h"

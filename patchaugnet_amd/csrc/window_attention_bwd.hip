@@ -16,7 +16,7 @@
 // is applied to the 32-bit sums, so that dS is rounded before it gets smaller.  delta takes o as the forward pass had it before it was rounded
 // (out + low): dP - delta is small beside delta, and with the rounded o alone dq and dk were off by 1.6 times the rounding of the result, now 1.42 to 1.47.
 //
-// Measured, dq / dk and dv / join: bf16 4 x 4096 tokens, 16 heads of 64 over 4, window 512: 77 / 113 / 5 us (630 / 575 TFLOP/s of visible pairs); all keys of
+// Measured, dq / dk and dv / join: bf16 4 x 4096 tokens, 16 heads of 64 over 4, window 512: 81 / 113 / 5 us (600 / 575 TFLOP/s of visible pairs); all keys of
 // 4 x 2048, 16 heads of 64: 114 / 157 us (900 / 870; a library product: 1219); 2 x 8192, 16 of 128 over 4, window 1024: 215 / 466 / 7 us; float32
 // 18 x 1024, 8 heads of 32, 128 keys either side: 109 / 155 / 9 us.  Bound by MFMA and LDS reads together (16 KB read for 16 to 32 products of a wave).
 // dk, dv at width 128 holds 390 registers, one wave per SIMD: there nothing hides a wave's exponentials, and its rate is 550.
