@@ -274,3 +274,20 @@ def test_keys_behind_four_gigabytes():
     for n in ("dk", "dv"):
         close(got[n][:, near], val[n], tol[n], n)
         assert int(got[n].count_nonzero()) == int(got[n][:, near].count_nonzero())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("N,H,Hk,D,left,sinks,few", [
+    (2, 2, 2, 32, None, 0, True), (3, 4, 1, 64, None, 0, True), (90, 8, 2, 64, 16, 1, True), (300, 4, 4, 128, None, 0, True), (300, 4, 2, 16, 40, 2, True),
+    (2100, 4, 2, 64, 511, 4, False), (2100, 4, 2, 128, 511, 4, False), (2100, 4, 2, 16, 511, 4, False)])
+def test_error_beside_the_rounding_of_the_result(dtype, N, H, Hk, D, left, sinks, few):
+    """2-norm of the error over that of rounding the exact result.  Up to 2^22 pairs products take P and dS in two parts, whose remainder is 2^-8 of a rounding or
+    less: even magnified ten times by the difference in dS it adds 1e-3 in the sum of squares.  Above, the rounding of P counts once in out and dv (sqrt 2), that
+    of dS once and that of P, through delta, at most once more in dq and dk (sqrt 3): independent errors of the rounding's relative size.  2 % for the sample."""
+    assert few == (H * N * min(N, N if left is None else left + 1) <= 1 << 22)
+    q, k, v, do = _qkv(1, N, N, H, Hk, D, dtype, seed=11)
+    got = _run(q, k, v, do, left, 0, sinks)
+    val, _ = reference(q, k, v, left, 0, sinks, None, None, None, do)
+    for n, most in (("out", 2), ("dq", 3), ("dk", 3), ("dv", 2)):
+        ratio = (got[n].double() - val[n]).norm() / (val[n].to(dtype).double() - val[n]).norm()
+        assert ratio <= 1.02 * (1 if few else most) ** 0.5, (n, float(ratio))
