@@ -48,6 +48,10 @@ void pa_emd_persistent_enable(int on);
 void pa_fpx16_enable(int mode);
 void pa_tgemm_cm_enable(int on);
 
+/* Floats of scratch that the launches of pa_window_attention_backward touch at these sizes (started: with a `start` array): host arithmetic only, held
+ * by the tests against what pa_window_attention_backward_scratch_floats promises. */
+long pa_window_attention_backward_plan_floats(int dtype, int b, int n, int m, int h, int hk, int d, int left, int right, int sinks, int started);
+
 #ifdef __cplusplus
 }
 #endif

@@ -432,7 +432,7 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int 
     if (n > walk / 4) n = walk / 4;
     s.slices = n < 1 ? 1 : n > 64 ? 64 : (int)n;
     const int first = sinks < M ? sinks : M;
-    const bool far = first > 0 && (started ? left < M : left < N - 1);          // rows behind the window of the first tokens
+    const bool far = N > 0 && first > 0 && (started ? left < M : left < N - 1);        // rows behind the window of the first tokens
     s.groups = far ? pa_div_up(first, 32) : 0;
     s.nst = pa_div_up(first, kb);
     long f = (rows + 16 * s.rt - 1) / (16 * s.rt);
@@ -492,6 +492,13 @@ PA_API long pa_window_attention_backward_scratch_floats(int b, int n, int m, int
     return pa_div_up((long)b * h * n, 4) * 4l + most * 2 * width(d);
 }
 
+PA_API long pa_window_attention_backward_plan_floats(int dtype, int b, int n, int m, int h, int hk, int d, int left, int right, int sinks, int started)
+{
+    const Shape s = shape_of(b, n, m, h, hk, d, dtype == PA_DT_F32 ? 4 : 2, left < 0 ? UNBOUNDED : left, right < 0 ? UNBOUNDED : right, sinks, started != 0);
+    const long slots = s.nkt ? s.slots((long)b * hk) : 0;
+    return (n > 0 || slots > 0 ? pa_div_up((long)b * h * n, 4) * 4l : 0) + slots * 2 * width(d);
+}
+
 PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb,
                                         long kn, long kh, const void *v, long vb, long vn, long vh, const void *out, const void *low, const float *lse, const void *dout, long gb,
                                         long gn, long gh, int left, int right, int sinks, float scale, const int *start, const int *length, void *dq, void *dk,
@@ -523,6 +530,7 @@ PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, i
     PA_REQUIRE(a.G <= 32 || (long)a.G * (qh > gh ? qh : gh) * 4 < (1l << 31), "pa_window_attention_backward: the heads of a group span 2^31 bytes");
     PA_REQUIRE((long)a.nqt * b * hk < (1l << 31) && (long)b * hk * ((long)s.groups * s.fars + (long)s.nkt * s.slices) * 128 < (1l << 31),
                "pa_window_attention_backward: too many workgroups");
+    PA_REQUIRE(s.slots((long)b * hk) == 0 || scratch, "pa_window_attention_backward: this size needs pa_window_attention_backward_scratch_floats() of scratch");
     hipStream_t st = (hipStream_t)stream;
 #define BWD(T, DT) launch_bwd<T, DT>(a, s, st)
     PA_ATTN_DISPATCH(dtype, d, BWD);

@@ -103,3 +103,19 @@ def test_misaligned_addresses_are_refused(lib):
         assert lib.pa_paged_attention(0, 1, 1, 1, 32, at, 0, 32, *bad, *z, 1, 1, at, 1, at, -1, 0, 1.0, at, at, p) == -1
         assert lib.pa_paged_append(0, 1, 1, 1, 32, *bad, *z, *z, *z, 1, 1, at, 1, at, p, p) == -1
         assert b"16 bytes" in lib.pa_last_error()
+
+
+def test_backward_scratch_holds_what_the_launches_touch(lib):
+    """Host arithmetic over small sizes, none of them left out: no queries, no keys, one of each; first tokens with and without rows behind their window."""
+    plan, promise = lib.pa_window_attention_backward_plan_floats, lib.pa_window_attention_backward_scratch_floats
+    plan.argtypes, plan.restype = [ctypes.c_int] * 11, ctypes.c_long
+    for n in (0, 1, 2, 63, 700):
+        for m in (0, 1, 5, 129, 900):
+            for h, hk in ((1, 1), (4, 2), (40, 1)):
+                for left, right in ((-1, 0), (0, 0), (3, 0), (200, 20)):
+                    for sinks in (0, 1, 33, 2000):
+                        for d in (8, 128):
+                            for dtype in (0, 1, 2):
+                                for started in (0, 1):
+                                    case = (dtype, 2, n, m, h, hk, d, left, right, sinks, started)
+                                    assert plan(*case) <= promise(*case[1:-1]), case

@@ -291,3 +291,13 @@ def test_error_beside_the_rounding_of_the_result(dtype, N, H, Hk, D, left, sinks
     for n, most in (("out", 2), ("dq", 3), ("dk", 3), ("dv", 2)):
         ratio = (got[n].double() - val[n]).norm() / (val[n].to(dtype).double() - val[n]).norm()
         assert ratio <= 1.02 * (1 if few else most) ** 0.5, (n, float(ratio))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_no_queries_behind_first_tokens(dtype):
+    """An empty part of a prompt: nothing sees the keys, their gradients are zeros whatever the window and the first tokens."""
+    for left, sinks, starts in ((3, 2, [4, 90]), (0, 40, [0, 0]), (None, 5, [7, 200])):
+        got = _run(*_qkv(2, 0, 90, 4, 2, 32, dtype), left, 0, sinks, lengths=[90, 41], starts=starts)
+        assert got["out"].shape == got["dq"].shape == (2, 0, 4, 32)
+        for n in ("dk", "dv"):
+            assert got[n].shape == (2, 90, 2, 32) and not got[n].any()
