@@ -76,7 +76,7 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
     {
         const T *qp = (const T *)a.q + b * a.qb + i * a.qn + hq * a.qh;
 #pragma unroll
-        for (int kk = 0; kk < DT / 16; ++kk) qf[kk] = ldrow<T>(qp, kk, h, a.D, row < rows);
+        for (int kk = 0; kk < DT / 16; ++kk) qf[kk] = ldrow<T>(qp, kk, h, a.D, keys.ok);        // padding rows are zeros
     }
     // the wave's rows: positions of the first and of the last one that is not padding
     const int wr = __builtin_amdgcn_readfirstlane(r0 + wave * 32);
@@ -171,7 +171,8 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
         }
         return;
     }
-    const float inv = keys.ok && l_run != 0.f ? 1.0f / l_run : 0.f;         // padding rows computed on zeros: their output is 0
+    const bool some = keys.ok && l_run != 0.f;                 // padding rows take part where their wave's other rows see everything: 0, whatever came out
+    const float inv = 1.0f / l_run;
     const size_t place = (((size_t)b * a.N + i) * a.H + hq) * a.D;
     T *op = (T *)a.out + place, *low = a.low ? (T *)a.low + place : nullptr;
 #pragma unroll
@@ -179,9 +180,11 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void fwd_kernel
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int c = ct * 32 + 8 * u + 4 * h;
-            if (c < a.D) store_out<T>(op + c, low ? low + c : nullptr, (pa_f4){o[ct][4 * u] * inv, o[ct][4 * u + 1] * inv, o[ct][4 * u + 2] * inv, o[ct][4 * u + 3] * inv});
+            pa_f4 x = (pa_f4)(0.f);
+            if (some) x = (pa_f4){o[ct][4 * u] * inv, o[ct][4 * u + 1] * inv, o[ct][4 * u + 2] * inv, o[ct][4 * u + 3] * inv};
+            if (c < a.D) store_out<T>(op + c, low ? low + c : nullptr, x);
         }
-    if (a.lse && h == 0) a.lse[((size_t)b * a.H + hq) * a.N + i] = inv == 0.f ? INFINITY : m_run + __builtin_amdgcn_logf(l_run);
+    if (a.lse && h == 0) a.lse[((size_t)b * a.H + hq) * a.N + i] = some ? m_run + __builtin_amdgcn_logf(l_run) : INFINITY;
 }
 
 // The rows of a split launch: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  A thread owns four elements of a row.
@@ -208,10 +211,12 @@ __global__ __launch_bounds__(256) void join_kernel(const FwdArgs a)
     }
     const int bh = (int)(at / rows), row = (int)(at - (size_t)bh * rows), b = bh / a.Hk, hk = bh - b * a.Hk;
     const int i = a.g.div(row), hq = hk * a.G + row - i * a.G;
-    const float inv = a.view.first(b) + i < a.view.len(b) && l != 0.f ? 1.0f / l : 0.f;
+    const bool some = a.view.first(b) + i < a.view.len(b) && l != 0.f;      // padding rows: 0
+    if (some) o *= 1.0f / l;
+    else o = (pa_f4)(0.f);
     const size_t place = (((size_t)b * a.N + i) * a.H + hq) * a.D + c;
-    if (c < a.D) store_out<T>((T *)a.out + place, a.low ? (T *)a.low + place : nullptr, o * inv);
-    if (a.lse && c == 0) a.lse[((size_t)b * a.H + hq) * a.N + i] = inv == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (c < a.D) store_out<T>((T *)a.out + place, a.low ? (T *)a.low + place : nullptr, o);
+    if (a.lse && c == 0) a.lse[((size_t)b * a.H + hq) * a.N + i] = some ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
 struct Shape {

@@ -147,7 +147,11 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
     }
     if (row >= rows) return;
     T *dp = (T *)a.dq + (((size_t)b * a.N + i) * a.H + hq) * a.D;
-    const float f = keys.ok ? a.scale : 0.f;
+    if (!keys.ok) {                                            // padding rows: 0, whatever the sequence's keys hold
+#pragma unroll
+        for (int ct = 0; ct < DT / 32; ++ct) dq[ct] = (pa_f16v)(0.f);
+    }
+    const float f = a.scale;
 #pragma unroll
     for (int ct = 0; ct < DT / 32; ++ct)
 #pragma unroll
@@ -343,6 +347,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
         if (t + 1 < t1) step(t + 1, q1, g1, r1, q0, g0);
     }
     if (w.far && j >= a.view.sinks) return;                     // nobody reads those
+    if (j >= len) {                                             // padding keys: 0, whatever the sequence's rows hold
+#pragma unroll
+        for (int ct = 0; ct < DT / 32; ++ct) dk[ct] = dv[ct] = (pa_f16v)(0.f);
+    }
     if (w.slot >= 0) {
         float *po = a.part + ((size_t)w.slot + wave * 32 + (l & 31)) * (2 * DT);
 #pragma unroll

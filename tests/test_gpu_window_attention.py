@@ -301,3 +301,27 @@ def test_no_queries_behind_first_tokens(dtype):
         assert got["out"].shape == got["dq"].shape == (2, 0, 4, 32)
         for n in ("dk", "dv"):
             assert got[n].shape == (2, 90, 2, 32) and not got[n].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("N,M,lengths,starts,left,right", [
+    (100, 100, [65, 3, 0, 100], None, None, 0), (100, 100, [65, 33, 97, 99], None, None, None), (300, 300, [257, 140, 70, 1], None, 200, 40),
+    (40, 3000, [3000, 2999, 2961, 5], [2980, 2960, 2960, 0], None, 0)])
+def test_padding_beside_rows_that_see_whole_parts(dtype, N, M, lengths, starts, left, right):
+    """Padding rows in a wave whose other rows see every key of a 32-key part; the last case splits the keys.  Padding of any value changes nothing, and where
+    the sequence itself holds NaN, the padding's output and gradients are still 0."""
+    q, k, v, do = _qkv(4, N, M, 4, 2, 64, dtype, seed=5)
+    ends = [max(n - (starts[b] if starts else 0), 0) for b, n in enumerate(lengths)]
+    clean = _run(q, k, v, do, left, right, 2, lengths, starts)
+    for b, n in enumerate(lengths):
+        q[b, ends[b]:], do[b, ends[b]:] = float("nan"), float("-inf")
+        k[b, n:], v[b, n:] = float("inf"), float("nan")
+    dirty = _run(q, k, v, do, left, right, 2, lengths, starts)
+    for n in clean:
+        assert torch.equal(clean[n], dirty[n]), n
+    v[0, 1], k[1, 2], do[2, 0] = float("nan"), float("inf"), float("inf")
+    broken = _run(q, k, v, do, left, right, 2, lengths, starts)
+    for got in (dirty, broken):
+        for b, n in enumerate(lengths):
+            assert not got["out"][b, ends[b]:].any() and not got["dq"][b, ends[b]:].any()
+            assert not got["dk"][b, n:].any() and not got["dv"][b, n:].any()
