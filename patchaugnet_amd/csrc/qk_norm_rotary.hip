@@ -136,25 +136,36 @@ template <int V> __device__ __forceinline__ void rotate(float *x, const Unit<V, 
 __device__ __forceinline__ int skip(int e) { return e + (e >> 4); }
 
 // The rotation where the pairs' second halves do not start at a whole piece: lanes keep pieces of consecutive elements, every element's partner comes
-// through the row's place in LDS.  A row is a wave's own, so LDS serves its stores and loads in order.
-template <int V> __device__ __forceinline__ void exchange(float *x, const Unit<V, true> &t, const NormArgs &a, float *row, const float *cs, const float *sn, float sign)
+// through the row's place in LDS.  A row is a wave's own, so LDS serves its stores and loads in order: first the pieces of all its units, then the partners
+// (a partner may lie in another unit of a lane).
+template <int V, int UPL> __device__ __forceinline__ void exchange(float (&x)[UPL][2 * V], const NormArgs &a, int lane, float *row, const float *cs, const float *sn, float sign)
 {
-    int e0 = t.o1;
-    asm volatile("" : "+v"(e0));                                // the places are worked out here, not kept for 2 V elements over all rows
-    if (t.on) {
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) row[skip(e0 + i)] = x[i];
+    for (int p = 0; p < UPL; ++p) {
+        const Unit<V, true> t(a, lane + p * a.lpr);
+        int e0 = t.o1;
+        asm volatile("" : "+v"(e0));                            // the places are worked out here, not kept for 2 V elements over all rows
+        if (t.on) {
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) row[skip(e0 + i)] = x[p][i];
+        }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (t.on) {
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) {
-            const int e = e0 + i;
-            const bool first = a.interleaved ? (e & 1) == 0 : e < a.pairs;
-            const int other = a.interleaved ? e ^ 1 : first ? e + a.pairs : e - a.pairs, p = a.interleaved ? e >> 1 : first ? e : other;
-            if (e < 2 * a.pairs) {
-                const float y = row[skip(other)], c = cs[skip(p)], s = sign * sn[skip(p)];
-                x[i] = first ? x[i] * c - y * s : y * s + x[i] * c;
+    for (int p = 0; p < UPL; ++p) {
+        const Unit<V, true> t(a, lane + p * a.lpr);
+        int e0 = t.o1;
+        asm volatile("" : "+v"(e0));
+        if (t.on) {
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) {
+                const int e = e0 + i;
+                const bool first = a.interleaved ? (e & 1) == 0 : e < a.pairs;
+                const int other = a.interleaved ? e ^ 1 : first ? e + a.pairs : e - a.pairs, pr = a.interleaved ? e >> 1 : first ? e : other;
+                if (e < 2 * a.pairs) {
+                    const float y = row[skip(other)], c = cs[skip(pr)], s = sign * sn[skip(pr)];
+                    x[p][i] = first ? x[p][i] * c - y * s : y * s + x[p][i] * c;
+                }
             }
         }
     }
@@ -220,22 +231,24 @@ __device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int
         const float r = rsqrt32(__builtin_fmaf(ss, inv_d, a.eps));
         if (!BWD) {
 #pragma unroll
-            for (int p = 0; p < UPL; ++p) {
-                const Unit<V, EX> t(a, lane + p * a.lpr);
+            for (int p = 0; p < UPL; ++p)
 #pragma unroll
                 for (int i = 0; i < 2 * V; ++i) v[p][i] = v[p][i] * r * w[p][i];
-                if constexpr (EX) exchange<V>(v[p], t, a, mine, cs, sn, 1.f);
-                else rotate<V>(v[p], t, a.interleaved, cs, sn, 1.f);
+            if constexpr (EX) exchange<V>(v, a, lane, mine, cs, sn, 1.f);
+#pragma unroll
+            for (int p = 0; p < UPL; ++p) {
+                const Unit<V, EX> t(a, lane + p * a.lpr);
+                if constexpr (!EX) rotate<V>(v[p], t, a.interleaved, cs, sn, 1.f);
                 if (t.on) store<T, V>(cur.y + t.o1, &v[p][0]);
                 if (t.two) store<T, V>(cur.y + t.o2, &v[p][V]);
             }
         } else {
             float dot = 0.f;
+            if constexpr (EX) exchange<V>(gr, a, lane, mine, cs, sn, -1.f);
 #pragma unroll
             for (int p = 0; p < UPL; ++p) {
                 const Unit<V, EX> t(a, lane + p * a.lpr);
-                if constexpr (EX) exchange<V>(gr[p], t, a, mine, cs, sn, -1.f);
-                else rotate<V>(gr[p], t, a.interleaved, cs, sn, -1.f);
+                if constexpr (!EX) rotate<V>(gr[p], t, a.interleaved, cs, sn, -1.f);
 #pragma unroll
                 for (int i = 0; i < 2 * V; ++i) {
                     v[p][i] *= r;                               // n

@@ -278,3 +278,27 @@ def test_positions_of_one_token():
     for pos in (torch.tensor([5], device="cuda"), torch.tensor([[5]], device="cuda"), torch.tensor([[[5]], [[5]]], device="cuda")):
         got = qk_norm_rotary(q, k, positions=pos, inv_freq=fr.view(-1) if pos.dim() == 1 else fr)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D,P", [(260, 129), (300, 149), (300, 3), (508, 253), (508, 127)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_exchanged_pairs_of_wide_heads(dtype, D, P, inter):
+    """Rows of more than 64 pieces, two to a lane: a pair's halves lie in different pieces of the lanes."""
+    _check(1, 150, 3, 1, D, dtype, freq=_freq(1, P), pos=torch.arange(150, device="cuda", dtype=torch.int32), inter=inter, seed=D + P)
+
+
+@pytest.mark.parametrize("dtype,shift", [(F32, 2), (F16, 2), (BF16, 2), (F32, 1), (BF16, 1)])
+@pytest.mark.parametrize("P", [255, 201, 66])
+def test_offset_views_of_wide_heads(dtype, shift, P):
+    """Rows of 512 that start at 8 or 4 bytes (float32), 4 or 2 bytes (16-bit): narrower pieces, up to four to a lane."""
+    from patchaugnet_amd.attention import qk_norm_rotary
+    g = torch.Generator(device="cuda").manual_seed(P)
+    wide, dy = (torch.randn(2, 40, 3, w, generator=g, device="cuda").to(dtype) for w in (512 + shift, 512))
+    q = wide[..., shift:].detach().requires_grad_()
+    pos, fr = torch.arange(40, device="cuda"), _freq(1, P)
+    out = qk_norm_rotary(q, q.detach(), positions=pos, inv_freq=fr)
+    (dq,) = torch.autograd.grad(out[0], q, dy)
+    want = _reference(q.detach(), None, *_angles(pos, fr, 2, 40), 1e-6, False, dy)
+    for got, n in ((out[0].detach(), "y"), (out[1], "y"), (dq, "dx")):
+        _close(got, want[n], n)
