@@ -293,8 +293,8 @@ def window_attention(q, k, v, *, left=None, right=0, sinks=0, scale=None, length
       q_start   int32 (B,): position of the first query (None: 0) -- the next part of a prompt, whose earlier keys lie in front of it in k and v.
     Values outside 0..M are clamped.  scale None: 1 / sqrt(D).  Strides are free except that a row is contiguous and starts at a multiple of 16 bytes
     (other tensors are copied; so are those with 2^22 elements and more between two tokens).  Gradients for q, k, v, the same bits on every run; in the
-    16-bit types what the rounding of out left, a tensor of its size, is kept for them.  float16: the gradient of a score, before `scale`, is held in that
-    type too, so what passes 65504 there comes out as no number."""
+    16-bit types what the rounding of out left, a tensor of its size, is kept for them.  Weights and the gradients of scores are rounded to the tensors' type
+    for the products; float16: brought into its range by powers of two first, so neither small gradients nor those that pass 65504 there are lost."""
     name = "window_attention"
     _check(name, q, k, v)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:

@@ -29,10 +29,23 @@ namespace {
 // dk, dv: rows of a tile, fewer where they are wide (registers on their way into LDS)
 template <typename T, int DT> constexpr int row_tile() { return DT * (int)sizeof(T) >= 512 ? 32 : 64; }
 
+// float16 has its full digits from 2^-14 to 65504.  P, about 1 / keys, and dS, which has the size of the incoming gradient besides, are lifted by powers of
+// two before they are packed, and the 32-bit sums are brought back.  In dv P takes 2^12 (a factor of 2^3 is left for what the rounding of a large lse
+// adds).  In dq a row's factor puts its first |dS| below 2^10 and is lowered when one passes 2^15, like the running maximum of the forward pass; the largest
+// |dS| of every 32 rows is left for dk, where the rows that a workgroup walks share the factor that puts the largest of them below 2^15.  So dS keeps all digits
+// down to 2^-24 of the largest one of its row (dq), 2^-28 of the largest one in its workgroup's rows (dk).
+template <typename T> constexpr bool lifted() { return false; }
+template <> constexpr bool lifted<_Float16>() { return true; }
+constexpr float P_LIFT = 12.f;
+constexpr int MAX_LIFT = 80;           // 2^80 times the largest dP - delta (2^39) stays inside 32 bits' exponents
+
+__device__ __forceinline__ float pow2(int e) { return __builtin_ldexpf(1.f, e); }
+__device__ __forceinline__ int exponent(float x) { return __builtin_amdgcn_frexp_expf(x); }        // x in [2^(e-1), 2^e)
+
 struct BwdArgs {
     const void *q, *k, *v, *out, *low, *dout;
     const float *lse;
-    float *delta, *part;
+    float *delta, *peak, *part;         // peak: largest |dS| of every 32 rows (float16)
     void *dq, *dk, *dv;
     long qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh;
     int B, N, H, Hk, D, G, nqt;
@@ -103,6 +116,8 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
     pa_f16v dq[DT / 32];
 #pragma unroll
     for (int ct = 0; ct < DT / 32; ++ct) dq[ct] = (pa_f16v)(0.f);
+    int e = 0;                                                 // lifted types: sums are 2^e dq, most the largest |2^e dS| so far
+    float f = 1.f, fdelta = delta, most = 0.f, top = 0.f;
 
     const TileList<KT> tiles(a.view, start + a.g.div(r0), start + a.g.div(min(r0 + QT, rows) - 1), len);
     if (tiles.n) fetch(tiles.tile(0), k0, v0);
@@ -126,7 +141,29 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
 #pragma unroll
             for (int kk = 0; kk < DT / 16; ++kk) mma(dp, L::ld(vs, sub * 32, kk), gf[kk]);              // meanwhile the exponentials
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = ex2(__builtin_fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
+            for (int r = 0; r < 16; ++r) s[r] = ex2(__builtin_fmaf(s[r], a.c, -lse)) * (lifted<T>() ? __builtin_fmaf(dp[r], f, -fdelta) : dp[r] - delta);
+            if constexpr (lifted<T>()) {
+                float mx = fabsf(s[0]);
+#pragma unroll
+                for (int r = 1; r < 16; ++r) mx = larger(mx, fabsf(s[r]));
+                mx = larger(mx, other_half(mx));
+                most = fmaxf(most, mx);
+                if (__any(mx > top)) {                         // the first dS that is not 0, or one that passes 2^15
+                    const int up = mx > top ? min(e + 10 - exponent(mx), MAX_LIFT) : e;
+                    const float by = pow2(up - e);
+#pragma unroll
+                    for (int ct = 0; ct < DT / 32; ++ct)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) dq[ct][r] *= by;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] *= by;
+                    top = mx > top ? 0x1p15f : top;
+                    most *= by;
+                    e = up;
+                    f = pow2(e);
+                    fdelta = delta * f;
+                }
+            }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const F ds = pack<T>(s, u);
@@ -145,19 +182,25 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
         step(it, k0, v0, k1, v1);
         if (it + 1 < tiles.n) step(it + 1, k1, v1, k0, v0);
     }
+    if constexpr (lifted<T>()) {
+        most *= pow2(-e);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+        if (l == 0) a.peak[((size_t)bh * a.nqt + qt) * NW + wave] = most;
+    }
     if (row >= rows) return;
     T *dp = (T *)a.dq + (((size_t)b * a.N + i) * a.H + hq) * a.D;
     if (!keys.ok) {                                            // padding rows: 0, whatever the sequence's keys hold
 #pragma unroll
         for (int ct = 0; ct < DT / 32; ++ct) dq[ct] = (pa_f16v)(0.f);
     }
-    const float f = a.scale;
+    const float back = lifted<T>() ? a.scale * pow2(-e) : a.scale;
 #pragma unroll
     for (int ct = 0; ct < DT / 32; ++ct)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int c = ct * 32 + 8 * u + 4 * h;
-            if (c < a.D) st4<T>(dp + c, dq[ct][4 * u] * f, dq[ct][4 * u + 1] * f, dq[ct][4 * u + 2] * f, dq[ct][4 * u + 3] * f);
+            if (c < a.D) st4<T>(dp + c, dq[ct][4 * u] * back, dq[ct][4 * u + 1] * back, dq[ct][4 * u + 2] * back, dq[ct][4 * u + 3] * back);
         }
 }
 
@@ -222,6 +265,20 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
     const int all = (rb - ra + a.rt - 1) / a.rt;
     const int t0 = (int)((long)all * w.slice / w.slices), t1 = (int)((long)all * (w.slice + 1) / w.slices);
 
+    int e = 0;                                                 // lifted types: sums are 2^e dk and 2^P_LIFT dv
+    if constexpr (lifted<T>()) {
+        if (t0 < t1) {
+            const float *peak = a.peak + (size_t)w.bh * a.nqt * 4;       // of the four waves of the dq launch's workgroups
+            float most = 0.f;
+            const int last = (min(ra + t1 * a.rt, rb) - 1) / 32;
+            for (int x = (ra + t0 * a.rt) / 32 + l; x <= last; x += 64) most = fmaxf(most, peak[x]);
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+            e = most > 0.f ? min(15 - exponent(most), MAX_LIFT) : 0;
+        }
+    }
+    const float f = lifted<T>() ? pow2(e - (int)P_LIFT) : 1.f;
+
     const int wk = __builtin_amdgcn_readfirstlane(w.far ? w.k0 : w.k0 + wave * 32), wk1 = min(wk + 31, len - 1);
     const bool wave_on = wk < len;
     const int j = wk + (l & 31);
@@ -267,8 +324,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
                 hq = hk * a.G + first + tid - i * a.G;
             }
             const size_t at = ((size_t)b * a.H + hq) * a.N + i;
-            pl = tid < valid ? a.lse[at] : INFINITY;
-            pd = tid < valid ? a.delta[at] : 0.f;
+            pl = tid < valid ? a.lse[at] - (lifted<T>() ? P_LIFT : 0.f) : INFINITY;
+            pd = tid < valid ? a.delta[at] * f : 0.f;
             pp = start + i;
         }
     };
@@ -315,10 +372,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
                 const int rr = sub * 32 + 8 * u + 4 * h;
                 const pa_f4 lse = *reinterpret_cast<const pa_f4 *>(ls + rr), delta = *reinterpret_cast<const pa_f4 *>(ds + rr);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * u + e;
-                    s[r] = ex2(__builtin_fmaf(s[r], a.c, -lse[e]));
-                    dp[r] = s[r] * (dp[r] - delta[e]);
+                for (int x = 0; x < 4; ++x) {
+                    const int r = 4 * u + x;
+                    s[r] = ex2(__builtin_fmaf(s[r], a.c, -lse[x]));
+                    dp[r] = s[r] * (lifted<T>() ? __builtin_fmaf(dp[r], f, -delta[x]) : dp[r] - delta[x]);
                 }
             }
 #pragma unroll
@@ -351,6 +408,16 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
 #pragma unroll
         for (int ct = 0; ct < DT / 32; ++ct) dk[ct] = dv[ct] = (pa_f16v)(0.f);
     }
+    if constexpr (lifted<T>()) {
+        const float bk = pow2(-e), bv = pow2(-(int)P_LIFT);
+#pragma unroll
+        for (int ct = 0; ct < DT / 32; ++ct)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                dk[ct][r] *= bk;
+                dv[ct][r] *= bv;
+            }
+    }
     if (w.slot >= 0) {
         float *po = a.part + ((size_t)w.slot + wave * 32 + (l & 31)) * (2 * DT);
 #pragma unroll
@@ -366,14 +433,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
     if (j >= a.view.m) return;
     const size_t at = (((size_t)b * a.view.m + j) * a.Hk + hk) * a.D;
     T *ko = (T *)a.dk + at, *vo = (T *)a.dv + at;
-    const float f = a.scale;
 #pragma unroll
     for (int ct = 0; ct < DT / 32; ++ct)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int c = ct * 32 + 8 * u + 4 * h;
             if (c < a.D) {
-                st4<T>(ko + c, dk[ct][4 * u] * f, dk[ct][4 * u + 1] * f, dk[ct][4 * u + 2] * f, dk[ct][4 * u + 3] * f);
+                st4<T>(ko + c, dk[ct][4 * u] * a.scale, dk[ct][4 * u + 1] * a.scale, dk[ct][4 * u + 2] * a.scale, dk[ct][4 * u + 3] * a.scale);
                 st4<T>(vo + c, dv[ct][4 * u], dv[ct][4 * u + 1], dv[ct][4 * u + 2], dv[ct][4 * u + 3]);
             }
         }
@@ -487,7 +553,9 @@ int launch_bwd(const BwdArgs &a, const Shape &s, hipStream_t st)
 
 }  // namespace
 
-// floats of scratch: delta (B H N), then the partial sums of sliced walks
+// floats of scratch: delta (B H N), the largest |dS| of every 32 rows, then the partial sums of sliced walks
+static long front_floats(int b, int n, int h, int hk) { return pa_div_up((long)b * h * n, 4) * 4l + (long)b * hk * pa_div_up((long)n * (h / hk), 128) * 4; }
+
 PA_API long pa_window_attention_backward_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks)
 {
     if (b <= 0 || n <= 0 || h <= 0 || hk <= 0 || h % hk != 0 || m < 0 || sinks < 0) return 0;
@@ -497,14 +565,14 @@ PA_API long pa_window_attention_backward_scratch_floats(int b, int n, int m, int
         const long k = shape_of(b, n, m, h, hk, d, i & 1 ? 4 : 2, left < 0 ? UNBOUNDED : left, right < 0 ? UNBOUNDED : right, sinks, i & 2).slots(bh);
         most = k > most ? k : most;
     }
-    return pa_div_up((long)b * h * n, 4) * 4l + most * 2 * width(d);
+    return front_floats(b, n, h, hk) + most * 2 * width(d);
 }
 
 PA_API long pa_window_attention_backward_plan_floats(int dtype, int b, int n, int m, int h, int hk, int d, int left, int right, int sinks, int started)
 {
     const Shape s = shape_of(b, n, m, h, hk, d, dtype == PA_DT_F32 ? 4 : 2, left < 0 ? UNBOUNDED : left, right < 0 ? UNBOUNDED : right, sinks, started != 0);
     const long slots = s.nkt ? s.slots((long)b * hk) : 0;
-    return (n > 0 || slots > 0 ? pa_div_up((long)b * h * n, 4) * 4l : 0) + slots * 2 * width(d);
+    return front_floats(b, n, h, hk) + slots * 2 * width(d);
 }
 
 PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, int hk, int d, const void *q, long qb, long qn, long qh, const void *k, long kb,
@@ -521,7 +589,8 @@ PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, i
     BwdArgs a;
     a.q = q; a.k = k; a.v = v; a.out = out; a.low = low; a.dout = dout; a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv;
     a.delta = scratch;
-    a.part = scratch + pa_div_up((long)b * h * n, 4) * 4l;
+    a.peak = scratch + pa_div_up((long)b * h * n, 4) * 4l;
+    a.part = scratch + front_floats(b, n, h, hk);
     a.qb = qb; a.qn = qn; a.qh = qh; a.kb = kb; a.kn = kn; a.kh = kh; a.vb = vb; a.vn = vn; a.vh = vh; a.gb = gb; a.gn = gn; a.gh = gh;
     a.B = b; a.N = n; a.H = h; a.Hk = hk; a.D = d; a.G = h / hk;
     a.view.m = m; a.view.left = left < 0 ? UNBOUNDED : left; a.view.right = right < 0 ? UNBOUNDED : right; a.view.sinks = sinks < m ? sinks : m;

@@ -325,3 +325,53 @@ def test_padding_beside_rows_that_see_whole_parts(dtype, N, M, lengths, starts, 
         for b, n in enumerate(lengths):
             assert not got["out"][b, ends[b]:].any() and not got["dq"][b, ends[b]:].any()
             assert not got["dk"][b, n:].any() and not got["dv"][b, n:].any()
+
+
+def _ratios(got, val, rows=slice(None)):
+    """2-norm of the error over that of rounding the exact result, over some rows (or keys)."""
+    out = {}
+    for n in val:
+        g, v = got[n][:, rows].double(), val[n][:, rows]
+        out[n] = float((g - v).norm() / (v.to(got[n].dtype).double() - v).norm())
+    return out
+
+
+@pytest.mark.parametrize("N,H,Hk,D,left,sinks,amp", [
+    (512, 2, 2, 64, None, 0, 1e-3), (512, 2, 1, 32, 100, 4, 1e-4), (2048, 4, 4, 64, None, 0, 1e-2), (2048, 4, 2, 64, None, 0, 1e-3), (4096, 2, 2, 128, None, 3, 1e-3),
+    (16384, 1, 1, 64, None, 0, 1.0), (16384, 1, 1, 64, None, 0, 1e-3), (16384, 1, 1, 16, None, 0, 1.0), (3000, 4, 2, 32, 1023, 40, 1e-3), (3000, 4, 1, 96, 300, 0, 1e-3)])
+def test_float16_keeps_digits_of_small_gradients(N, H, Hk, D, left, sinks, amp):
+    """Weights of 1 / keys and gradients as a mean loss gives them.  Bounds as in test_error_beside_the_rounding_of_the_result: powers of two that are taken off again
+    change no rounding."""
+    few = H * N * min(N, N if left is None else left + 1) <= 1 << 22
+    q, k, v, do = _qkv(1, N, N, H, Hk, D, F16, seed=11)
+    do = do * amp
+    got = _run(q, k, v, do, left, 0, sinks)
+    val, _ = reference(q, k, v, left, 0, sinks, None, None, None, do)
+    for (n, r), most in zip(_ratios(got, val).items(), (2, 3, 3, 2)):
+        assert r <= 1.02 * (1 if few else most) ** 0.5, (n, r)
+
+
+def test_float16_gradients_of_different_sizes():
+    """Rows whose gradients are 2^0 .. 2^-11 in turn keep the digits of their own dq; a second half of 2^-13 keeps those of its dk and dv."""
+    q, k, v, do = _qkv(1, 2048, 2048, 4, 2, 64, F16, seed=12)
+    size = 2.0 ** -(torch.arange(2048, device="cuda") % 12)
+    mixed = do * size.to(F16).view(1, -1, 1, 1)
+    got = _run(q, k, v, mixed, None, 0, 0)
+    val, _ = reference(q, k, v, None, 0, 0, None, None, None, mixed)
+    for first in (0, 6, 11):
+        r = _ratios({"dq": got["dq"]}, {"dq": val["dq"]}, slice(first, None, 12))["dq"]
+        assert r <= 1.02 * 3 ** 0.5, (first, r)
+    halves = do * torch.where(torch.arange(2048, device="cuda") < 1024, 1.0, 2.0 ** -13).to(F16).view(1, -1, 1, 1)
+    got = _run(q, k, v, halves, 600, 0, 0)
+    val, _ = reference(q, k, v, 600, 0, 0, None, None, None, halves)
+    for part in (slice(0, 1024), slice(1024 + 128, 2048)):      # keys of the second half are seen by its rows alone
+        r = _ratios({n: got[n] for n in ("dk", "dv")}, {n: val[n] for n in ("dk", "dv")}, part)
+        assert r["dk"] <= 1.02 * 3 ** 0.5 and r["dv"] <= 1.02 * 2 ** 0.5, (part, r)
+
+
+@pytest.mark.parametrize("left,sinks", [(3, 0), (None, 2)])
+def test_float16_scores_gradients_beyond_its_range(left, sinks):
+    """dS of 10^6 and more (large values and gradients) beside keys and queries of 10^-3: the products fit the type, dS alone would not."""
+    q, k, v, do = _qkv(1, 200, 200, 4, 2, 32, F16, seed=13)
+    do[:, ::7] *= 2.0 ** -12                                    # and rows far below
+    _check(q * 2.0 ** -10, k * 2.0 ** -10, v * 64, do * 2.0 ** 13, left, 0, sinks)
