@@ -90,9 +90,11 @@ def _unit(t):
 
 
 def _strides(t):
-    """Strides of all dimensions but the last; 0 where a dimension has one entry (its stride is never used and may be anything)."""
+    """Strides of all dimensions but the last.  A dimension with one entry may report any stride, in contiguous tensors too; the library would hold that
+    against its limits, so it gets the stride of the shape, or 0."""
     if t.is_contiguous():
-        return t.stride()[:-1]
+        n = t.shape
+        return (n[1] * n[2] * n[3], n[2] * n[3], n[3]) if len(n) == 4 else (n[1] * n[2], n[2])
     return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
 
 
@@ -292,7 +294,7 @@ def window_attention(q, k, v, *, left=None, right=0, sinks=0, scale=None, length
                 q, k, v holds has no influence, NaN included.  Within a sequence a NaN or an infinity reaches rows that do not see it.
       q_start   int32 (B,): position of the first query (None: 0) -- the next part of a prompt, whose earlier keys lie in front of it in k and v.
     Values outside 0..M are clamped.  scale None: 1 / sqrt(D).  Strides are free except that a row is contiguous and starts at a multiple of 16 bytes
-    (other tensors are copied; so are those with 2^22 elements and more between two tokens).  Gradients for q, k, v, the same bits on every run; in the
+    (other tensors are copied; so are those with 2^22 elements and more between two tokens or heads; H D up to 2^22).  Gradients for q, k, v, the same bits on every run; in the
     16-bit types what the rounding of out left, a tensor of its size, is kept for them.  Weights and the gradients of scores are rounded to the tensors' type
     for the products; float16: brought into its range by powers of two first, so neither small gradients nor those that pass 65504 there are lost."""
     name = "window_attention"

@@ -242,3 +242,18 @@ def test_refusals():
             bad()
     with torch.no_grad():
         paged_attention(q.clone().requires_grad_(), kp, vp, table, ln)
+
+
+def test_strides_of_dimensions_with_one_entry_mean_nothing():
+    from patchaugnet_amd.attention import paged_append, paged_attention
+    q, k, v = _inputs(1, 40, 1, 1, 32, BF16, seed=2)
+    kp, vp, table = _cache(k, v, 40, [40], spare=0)
+    want = paged_attention(q, kp, vp, table, _i([40]))
+
+    def odd(t):
+        return t.as_strided(t.shape, tuple(s if n > 1 else 13 for s, n in zip(t.stride(), t.shape)))
+
+    assert odd(kp).stride(0) == 13 and odd(kp).is_contiguous()
+    assert torch.equal(want, paged_attention(odd(q), odd(kp), odd(vp), table, _i([40])))
+    paged_append(odd(v[:, 3:4]), odd(k[:, 3:4]), odd(kp), odd(vp), table, _i([7]))
+    assert torch.equal(kp[0, 7], v[0, 3]) and torch.equal(vp[0, 7], k[0, 3])

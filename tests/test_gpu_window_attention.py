@@ -375,3 +375,25 @@ def test_float16_scores_gradients_beyond_its_range(left, sinks):
     q, k, v, do = _qkv(1, 200, 200, 4, 2, 32, F16, seed=13)
     do[:, ::7] *= 2.0 ** -12                                    # and rows far below
     _check(q * 2.0 ** -10, k * 2.0 ** -10, v * 64, do * 2.0 ** 13, left, 0, sinks)
+
+
+def test_strides_of_dimensions_with_one_entry_mean_nothing():
+    """One batch, one token, one head: their strides may be anything, a single head cut out of (B, H, N, D) among them."""
+    q, k, v, do = _qkv(1, 50, 50, 1, 1, 32, BF16, seed=1)
+    want = _run(q, k, v, do, 9, 0, 1)
+    odd = [t.as_strided(t.shape, s) for t, s in ((q, (1601, 32, 1 << 23, 1)), (k, (7, 32, 33, 1)), (v, (1, 32, 1 << 30, 1)), (do, (3, 32, 5, 1)))]
+    assert all(t.is_contiguous() for t in odd)
+    got = _run(*odd, 9, 0, 1)
+    for n in want:
+        assert torch.equal(want[n], got[n]), n
+    one = [t[:, :1] for t in (q, k, v, do)]
+    want = _run(*[t.contiguous() for t in one], None, 0, 0)
+    got = _run(*[t.as_strided(t.shape, (33, 1 << 23, 17, 1)) for t in one], None, 0, 0)
+    for n in want:
+        assert torch.equal(want[n], got[n]), n
+    N = (1 << 22) // 128 + 5                                    # the head's stride passes 2^22 elements
+    q, k, v, do = (torch.randn(1, 1, N, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)).to(BF16).transpose(1, 2) for i in range(4))
+    got = _run(q, k, v, do, 20, 0, 0)
+    want = _run(*[t.squeeze(2).unsqueeze(2).clone(memory_format=torch.contiguous_format) for t in (q, k, v, do)], 20, 0, 0)
+    for n in want:
+        assert torch.equal(want[n], got[n]), n
