@@ -294,6 +294,9 @@ template <typename T, int DT> constexpr int waves_per_simd() { return sizeof(T) 
 // 128 keys either side: forward 88 us, dq 121; with 32 keys 76 and 109).
 template <typename T, int DT, int NW> constexpr int key_tile() { return NW == 2 ? 32 : 64; }
 
+// a launch holds fewer than 2^32 threads along a dimension
+static inline bool launchable(long workgroups, int threads) { return workgroups < (1l << 32) / threads; }
+
 static inline int width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }      // padded head width
 
 }  // namespace pa_attn

@@ -26,6 +26,7 @@ namespace {
 
 enum { F32 = PA_DT_F32, F16 = PA_DT_F16, BF16 = PA_DT_BF16 };
 constexpr int MAXD = 512, MAXTOK = 16;
+constexpr long MAXTURNS = 1l << 22;    // workgroups of the forward pass (2^30 threads); more turns go round
 constexpr int MAXGROUPS = 768;         // workgroups of the backward pass: three per CU are resident at its registers, one round
 
 struct Side {                           // the queries, or the keys
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void norm_kernel(const NormArgs a
     }
     for (int t0 = blockIdx.x * a.tb; t0 < a.tokens; t0 += gridDim.x * a.tb) {
         const int nt = min(a.tokens - t0, a.tb);
-        if (BWD) __syncthreads();                               // readers of the previous turn's table and angles
+        if (t0 != (int)blockIdx.x * a.tb) __syncthreads();      // readers of the previous turn's table and angles
         if (tid < 4 * MAXTOK && (tid & (MAXTOK - 1)) < nt) {
             const int s = tid / (2 * MAXTOK), g = tid / MAXTOK & 1, tok = tid & (MAXTOK - 1), b = a.dn.div(t0 + tok), n = t0 + tok - b * a.N;
             const Side &sd = s ? a.side[1] : a.side[0];
@@ -470,8 +471,7 @@ PA_API int pa_qk_norm_rotary(int dtype, int b, int n, int h, int hk, int d, cons
     a.N = n; a.D = d; a.axes = axes; a.per = per; a.interleaved = interleaved; a.wtype = w_f32; a.ptype = ptype; a.eps = eps;
     const int es = dtype == F32 ? 4 : 2;
     const int v = norm_plan(a, dtype, b, false, alignment_of(es, {q, k, q_out, k_out}, {qb, qn, qh, kb, kn, kh, d}));
-    const long groups = (a.tokens + a.tb - 1) / a.tb;
-    PA_REQUIRE(groups < (1l << 31), "pa_qk_norm_rotary: too many workgroups");
+    const long turns = (a.tokens + a.tb - 1) / a.tb, groups = turns < MAXTURNS ? turns : MAXTURNS;
     const size_t lds = lds_of(a);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == F32) launch_norm<float, false>(a, v, dim3((unsigned)groups), lds, st);

@@ -298,7 +298,7 @@ PA_API int pa_window_attention(int dtype, int b, int n, int m, int h, int hk, in
     a.few = few_pairs((long)b * h, n, m, (long)a.view.left + a.view.right + 1);
     a.splits = sh.splits;
     PA_REQUIRE(kn >= 0 && vn >= 0 && kn <= PA_ATTN_MAXSTRIDE && vn <= PA_ATTN_MAXSTRIDE, "pa_window_attention: tokens are more than 2^22 elements apart");
-    PA_REQUIRE((long)a.nqt * b * hk < (1l << 31), "pa_window_attention: too many workgroups");
+    PA_REQUIRE(launchable((long)a.nqt * b * hk, 256), "pa_window_attention: too many workgroups");
     PA_REQUIRE(a.splits == 1 || scratch, "pa_window_attention: this size needs pa_window_attention_scratch_floats() of scratch");
     hipStream_t st = (hipStream_t)stream;
 #define FWD(T, DT) launch_fwd<T, DT>(a, st)

@@ -448,12 +448,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
 // dk, dv of the key tiles that left partial sums: the window's slices, then the far rows' (slice by slice, wave by wave).  A workgroup owns a key;
 // DT / 2 threads hold a row of dk and dv, four elements each, the 512 / DT groups of such threads take the sums in turn and are added in order.
 template <typename T, int DT, int NW>
-__global__ __launch_bounds__(256) void dkv_join_kernel(const BwdArgs a, int tiles)
+__global__ __launch_bounds__(256) void dkv_join_kernel(const BwdArgs a, int tiles, long first)
 {
     constexpr int C = DT / 2, P = 256 / C, KB = 32 * NW;
     __shared__ pa_f4 red[P][C];
     const int c = (int)threadIdx.x % C * 4, part = (int)threadIdx.x / C;
-    const long tile = blockIdx.x / KB;
+    const long tile = first + blockIdx.x / KB;
     const int r = (int)(blockIdx.x % KB);
     const int bh = (int)(tile / tiles), t = (int)(tile % tiles), b = bh / a.Hk, hk = bh - b * a.Hk, j = t * KB + r;
     if (j >= a.view.m) return;
@@ -527,7 +527,11 @@ void launch_dkv(const BwdArgs &a, int joined, hipStream_t st)
 {
     const long bh = (long)a.B * a.Hk;
     hipLaunchKernelGGL((dkv_kernel<T, DT, NW, FINE>), dim3((unsigned)(bh * a.groups * a.fars + bh * a.nkt * a.slices)), dim3(64 * NW), 0, st, a);
-    if (joined) hipLaunchKernelGGL((dkv_join_kernel<T, DT, NW>), dim3((unsigned)(bh * joined * 32 * NW)), dim3(256), 0, st, a, joined);
+    constexpr long most = (1l << 23) / (32 * NW);              // tiles of a launch: 2^31 threads
+    for (long first = 0; first < bh * joined; first += most) {
+        const long n = bh * joined - first < most ? bh * joined - first : most;
+        hipLaunchKernelGGL((dkv_join_kernel<T, DT, NW>), dim3((unsigned)(n * 32 * NW)), dim3(256), 0, st, a, joined, first);
+    }
 }
 
 template <typename T, int DT>
@@ -605,7 +609,7 @@ PA_API int pa_window_attention_backward(int dtype, int b, int n, int m, int h, i
                    gn <= PA_ATTN_MAXSTRIDE && qh <= PA_ATTN_MAXSTRIDE && gh <= PA_ATTN_MAXSTRIDE,
                "pa_window_attention_backward: tokens or heads are more than 2^22 elements apart");
     PA_REQUIRE(a.G <= 32 || (long)a.G * (qh > gh ? qh : gh) * 4 < (1l << 31), "pa_window_attention_backward: the heads of a group span 2^31 bytes");
-    PA_REQUIRE((long)a.nqt * b * hk < (1l << 31) && (long)b * hk * ((long)s.groups * s.fars + (long)s.nkt * s.slices) * 128 < (1l << 31),
+    PA_REQUIRE(launchable((long)a.nqt * b * hk, 256) && launchable((long)b * hk * ((long)s.groups * s.fars + (long)s.nkt * s.slices), 256),
                "pa_window_attention_backward: too many workgroups");
     PA_REQUIRE(s.slots((long)b * hk) == 0 || scratch, "pa_window_attention_backward: this size needs pa_window_attention_backward_scratch_floats() of scratch");
     hipStream_t st = (hipStream_t)stream;

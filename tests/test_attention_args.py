@@ -119,3 +119,19 @@ def test_backward_scratch_holds_what_the_launches_touch(lib):
                                 for started in (0, 1):
                                     case = (dtype, 2, n, m, h, hk, d, left, right, sinks, started)
                                     assert plan(*case) <= promise(*case[1:-1]), case
+
+
+def test_more_threads_than_a_launch_holds_are_refused(lib):
+    """Before anything runs (host addresses: the calls end there)."""
+    buf = (ctypes.c_char * 4096)()
+    base = (ctypes.addressof(buf) + 15) // 16 * 16
+    p, at, z = ctypes.c_void_p(0), ctypes.c_void_p(base), (ctypes.c_void_p(base), 0, 8, 8)
+    n = 2 ** 28
+    assert lib.pa_window_attention(2, 8, n, 4, 2, 1, 8, *z, *z, *z, -1, 0, 0, 1.0, p, p, at, p, p, at, p) == -1                # 2^32 rows
+    assert b"workgroups" in lib.pa_last_error()
+    assert lib.pa_window_attention_backward(2, 8, n, 4, 2, 1, 8, *z, *z, *z, at, p, at, *z, -1, 0, 0, 1.0, p, p, at, at, at, at, p) == -1
+    assert b"workgroups" in lib.pa_last_error()
+    assert lib.pa_window_attention_backward(0, 8, 4, n, 1, 1, 8, *z, *z, *z, at, p, at, *z, 0, 0, 0, 1.0, p, p, at, at, at, at, p) == -1      # 2^31 keys
+    assert b"workgroups" in lib.pa_last_error()
+    assert lib.pa_paged_attention(0, 2 ** 24, 1, 1, 8, at, 0, 8, *z, *z, 1, 1, at, 1, at, -1, 0, 1.0, at, at, p) == -1
+    assert b"workgroups" in lib.pa_last_error()

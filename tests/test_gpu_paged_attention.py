@@ -257,3 +257,15 @@ def test_strides_of_dimensions_with_one_entry_mean_nothing():
     assert torch.equal(want, paged_attention(odd(q), odd(kp), odd(vp), table, _i([40])))
     paged_append(odd(v[:, 3:4]), odd(k[:, 3:4]), odd(kp), odd(vp), table, _i([7]))
     assert torch.equal(kp[0, 7], v[0, 3]) and torch.equal(vp[0, 7], k[0, 3])
+
+
+def test_append_of_more_pieces_than_threads():
+    """2^31 pieces of 16 bytes and more, of one expanded row: all but the last tokens lie in front of the table."""
+    from patchaugnet_amd.attention import paged_append
+    T, Hk, D = (1 << 27) + 5, 8, 16
+    k = torch.randn(1, 1, Hk, D, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(BF16)
+    kp, vp = (torch.zeros(2, 4, Hk, D, dtype=BF16, device="cuda") for _ in range(2))
+    paged_append(k.expand(1, T, Hk, D), (-k).expand(1, T, Hk, D), kp, vp, _i([[1, 0]]), _i([3 - T]))
+    want = torch.zeros_like(kp)
+    want[1, :3] = k[0]
+    assert torch.equal(kp, want) and torch.equal(vp, -want)

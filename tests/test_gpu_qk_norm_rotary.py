@@ -302,3 +302,16 @@ def test_offset_views_of_wide_heads(dtype, shift, P):
     want = _reference(q.detach(), None, *_angles(pos, fr, 2, 40), 1e-6, False, dy)
     for got, n in ((out[0].detach(), "y"), (out[1], "y"), (dq, "dx")):
         _close(got, want[n], n)
+
+
+def test_more_turns_than_workgroups():
+    """2^26 tokens and some: the forward pass's workgroups take further turns; every token as in calls of 2^24."""
+    from patchaugnet_amd.attention import qk_norm_rotary
+    N = (1 << 26) + 100
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(1, N, 1, 8, generator=g, device="cuda", dtype=BF16)
+    pos, fr = torch.arange(N, device="cuda", dtype=torch.int32), _freq(1, 4)
+    whole = qk_norm_rotary(q, q[:, :N], positions=pos, inv_freq=fr)
+    for i in range(0, N, 1 << 24):
+        part = qk_norm_rotary(q[:, i:i + (1 << 24)], q[:, i:i + (1 << 24)], positions=pos[i:i + (1 << 24)], inv_freq=fr)
+        assert torch.equal(part[0], whole[0][:, i:i + (1 << 24)]) and torch.equal(part[1], whole[1][:, i:i + (1 << 24)]), i

@@ -397,3 +397,16 @@ def test_strides_of_dimensions_with_one_entry_mean_nothing():
     want = _run(*[t.squeeze(2).unsqueeze(2).clone(memory_format=torch.contiguous_format) for t in (q, k, v, do)], 20, 0, 0)
     for n in want:
         assert torch.equal(want[n], got[n]), n
+
+
+def test_more_joined_keys_than_a_launch_holds():
+    """2^24 first tokens and some, whose partial sums are joined by a workgroup each: the last ones come out like the first."""
+    M = (1 << 24) + 100
+    q, k, v, do = _qkv(1, 2, M, 1, 1, 8, BF16, seed=14)
+    do = do * 2.0 ** 10
+    got = _run(q, k, v, do, 0, None, M, lengths=[M], starts=[0])
+    val, _ = reference(q, k, v, 0, None, M, None, [M], [0], do)
+    for part in (slice(0, 4096), slice(M - 4096, M)):
+        for n in ("dk", "dv"):
+            assert val[n][:, part].any()
+            assert _ratios({n: got[n]}, {n: val[n]}, part)[n] <= 2.0, (n, part)
