@@ -173,14 +173,11 @@ template <int V, int UPL> __device__ __forceinline__ void exchange(float (&x)[UP
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-// 1 / sqrt(x): v_rsq_f32 and a Newton step; it flushes subnormal arguments, so small ones are lifted first
+// 1 / sqrt(x), 2^-126 <= x < 2^127: v_rsq_f32 and a Newton step
 __device__ __forceinline__ float rsqrt32(float x)
 {
-    const bool low = x < 0x1p-100f;
-    x = low ? x * 0x1p100f : x;
-    float r = __builtin_amdgcn_rsqf(x);
-    r = r * __builtin_fmaf(-0.5f * x * r, r, 1.5f);
-    return low ? r * 0x1p50f : r;
+    const float r = __builtin_amdgcn_rsqf(x);
+    return r * __builtin_fmaf(-0.5f * x * r, r, 1.5f);
 }
 
 // The rows of one side in a workgroup's turn of nt tokens from t0: row slot by row slot, the next one fetched while this one is computed.  where:
@@ -229,7 +226,21 @@ __device__ __forceinline__ void side_rows(const NormArgs &a, const Side &sd, int
                 ss = __builtin_fmaf(v[p][i], v[p][i], ss);
             }
         for (int o = 1; o < a.lpr; o <<= 1) ss += __shfl_xor(ss, o);
-        const float r = rsqrt32(__builtin_fmaf(ss, inv_d, a.eps));
+        float mean = __builtin_fmaf(ss, inv_d, a.eps), r = rsqrt32(mean);
+        if (!(mean >= 0x1p-100f && mean < 0x1p126f)) {          // squares that leave 32 bits: the root from the row times a power of two
+            const float lift = mean < 1.f ? 0x1p100f : 0x1p-75f;
+            ss = 0.f;
+#pragma unroll
+            for (int p = 0; p < UPL; ++p)
+#pragma unroll
+                for (int i = 0; i < 2 * V; ++i) {
+                    const float y = v[p][i] * lift;
+                    ss = __builtin_fmaf(y, y, ss);
+                }
+            for (int o = 1; o < a.lpr; o <<= 1) ss += __shfl_xor(ss, o);
+            mean = __builtin_fmaf(ss, inv_d, a.eps * lift * lift);
+            r = mean == INFINITY ? 0.f : rsqrt32(mean) * lift;
+        }
         if (!BWD) {
 #pragma unroll
             for (int p = 0; p < UPL; ++p)

@@ -315,3 +315,25 @@ def test_more_turns_than_workgroups():
     for i in range(0, N, 1 << 24):
         part = qk_norm_rotary(q[:, i:i + (1 << 24)], q[:, i:i + (1 << 24)], positions=pos[i:i + (1 << 24)], inv_freq=fr)
         assert torch.equal(part[0], whole[0][:, i:i + (1 << 24)]) and torch.equal(part[1], whole[1][:, i:i + (1 << 24)]), i
+
+
+@pytest.mark.parametrize("dtype,scale,eps", [(F32, 1e25, 1e-6), (BF16, 1e25, 1e-6), (F32, 3e37, 1e-6), (BF16, 1e19, 0.0), (F32, 1e-25, 0.0), (BF16, 1e-30, 0.0),
+                                             (F32, 1e-18, 1e-36), (F32, 1e-30, 1e-38)])
+def test_rows_whose_squares_leave_32_bits(dtype, scale, eps):
+    """Rows of 10^19 and more, and small ones under a small eps: the mean square is neither infinite nor 0.  Gradients of rows that large are below 32 bits' range."""
+    q, k = (torch.randn(2, 9, h, 48, generator=torch.Generator(device="cuda").manual_seed(h), device="cuda").mul(scale).to(dtype) for h in (3, 2))
+    from patchaugnet_amd.attention import qk_norm_rotary
+    pos, fr = torch.arange(9, device="cuda"), _freq(1, 8)
+    leaf, gy = q.clone().requires_grad_(), torch.randn(q.shape, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda").to(dtype)
+    out = qk_norm_rotary(leaf, k, positions=pos, inv_freq=fr, eps=eps)
+    (dq,) = torch.autograd.grad(out[0], leaf, gy)
+    want = _reference(q, None, *_angles(pos, fr, 2, 9), eps, False, gy)
+    _close(out[0].detach(), want["y"], "y")
+    _close(out[1], _reference(k, None, *_angles(pos, fr, 2, 9), eps, False)["y"], "k")
+    _close(dq, want["dx"], "dx")
+    mixed = q.clone()
+    mixed[0, 0, 0, 5], mixed[1, 2, 1, 3] = float("inf"), float("nan")
+    got = qk_norm_rotary(mixed, k, positions=pos, inv_freq=fr, eps=eps)[0]
+    other = torch.ones(q.shape[:3], dtype=torch.bool, device="cuda")
+    other[0, 0, 0] = other[1, 2, 1] = False
+    assert torch.equal(got[other], out[0].detach()[other]) and got[1, 2, 1].isnan().all()
