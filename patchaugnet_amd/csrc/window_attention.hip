@@ -235,7 +235,7 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int es, int left, int right, 
     const long wgs = (long)B * Hk * s.nqt;
     if (wgs >= 256) return s;
     const long span = (long)left + right + 32 * s.waves / G + 1;             // longest range of keys of one workgroup
-    const long tiles = pa_div_up(M < span ? M : span, 64) + (left < M ? pa_div_up(sinks, 64) : 0);
+    const long tiles = pa_div_up(M < span ? M : span, 64) + (left < M ? pa_div_up(sinks < M ? sinks : M, 64) : 0);
     const long want = 512 / wgs, most = tiles / 4;
     const long n = want < most ? want : most;
     s.splits = n < 1 ? 1 : (n > 64 ? 64 : (int)n);

@@ -135,3 +135,12 @@ def test_more_threads_than_a_launch_holds_are_refused(lib):
     assert b"workgroups" in lib.pa_last_error()
     assert lib.pa_paged_attention(0, 2 ** 24, 1, 1, 8, at, 0, 8, *z, *z, 1, 1, at, 1, at, -1, 0, 1.0, at, at, p) == -1
     assert b"workgroups" in lib.pa_last_error()
+
+
+def test_first_tokens_behind_the_last_key_ask_for_no_splits(lib):
+    """`sinks` beyond the keys means all of them, also where the work is cut."""
+    g = lib.pa_window_attention_scratch_floats
+    for n, m in ((64, 64), (3, 1000), (1, 5000), (40, 0)):
+        for left in (-1, 0, 16, 300):
+            assert g(1, n, m, 8, 8, 32, left, 0, 10 ** 6) == g(1, n, m, 8, 8, 32, left, 0, m), (n, m, left)
+    assert g(1, 64, 64, 8, 8, 32, 16, 0, 10 ** 6) == 0
