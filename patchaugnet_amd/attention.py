@@ -65,19 +65,24 @@ def _ints(name, what, t, device, n):
     return t.contiguous()
 
 
-def _rows(t, align=16, far=1 << 62):
-    """t itself if its last dimension is contiguous, every row starts at a multiple of `align` bytes and those of neighbouring tokens and heads lie at most
-    `far` elements apart, else a contiguous copy."""
+def _fits(t, align=16, far=1 << 62):
+    """Is the last dimension contiguous, does every row start at a multiple of `align` bytes, and do those of neighbouring tokens and heads lie at most `far`
+    elements apart?"""
     if t.is_contiguous():
-        return t if t.data_ptr() % align == 0 else t.clone()
+        return t.data_ptr() % align == 0
     s = t.stride()
     outer, es = 0, t.element_size()
     for i, n in zip(s[:-1], t.shape):
         if n > 1:
             outer |= i
-    if s[-1] == 1 and t.data_ptr() % align == 0 and outer * es % align == 0 and (far > _FAR or _near(t, s)):
+    return s[-1] == 1 and t.data_ptr() % align == 0 and outer * es % align == 0 and (far > _FAR or _near(t, s))
+
+
+def _rows(t, align=16, far=1 << 62):
+    """t itself if it fits, else a contiguous copy."""
+    if _fits(t, align, far):
         return t
-    return t.contiguous()
+    return t.clone() if t.is_contiguous() else t.contiguous()
 
 
 def _near(t, s):
@@ -318,7 +323,7 @@ def _cache(name, k_pages, v_pages, table, B):
     if k_pages.shape[1] < 1 or k_pages.shape[2] < 1:
         raise ValueError(f"{name}: empty pages or no key heads: {tuple(k_pages.shape)}")
     for t in (k_pages, v_pages):
-        if _rows(t) is not t and t.numel():
+        if not _fits(t) and t.numel():
             raise ValueError(f"{name}: a row of a page has to be contiguous and to start at a multiple of 16 bytes")
     if not isinstance(table, torch.Tensor) or table.dtype != torch.int32 or table.device != k_pages.device or table.dim() != 2 or table.shape[0] != B:
         raise ValueError(f"{name}: page_table has to be an int32 tensor (B, pages of a sequence) on {k_pages.device}, B = {B}")

@@ -269,3 +269,19 @@ def test_append_of_more_pieces_than_threads():
     want = torch.zeros_like(kp)
     want[1, :3] = k[0]
     assert torch.equal(kp, want) and torch.equal(vp, -want)
+
+
+def test_refused_pools_are_not_copied():
+    from patchaugnet_amd.attention import paged_append, paged_attention
+    q, k, v = _inputs(1, 16, 2, 2, 32, BF16)
+    flat = torch.zeros(4096 * 16 * 2 * 32 + 8, dtype=BF16, device="cuda")
+    shifted = flat[1:-7].view(4096, 16, 2, 32)
+    skew = torch.zeros(4096, 16, 2, 33, dtype=BF16, device="cuda")[..., 1:]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.max_memory_allocated()
+    for pool in (shifted, skew):
+        for call in (lambda: paged_attention(q, pool, pool, _i([[0]]), _i([16])), lambda: paged_append(k, v, pool, pool, _i([[0]]), _i([0]))):
+            with pytest.raises(ValueError, match="16 bytes"):
+                call()
+    assert torch.cuda.max_memory_allocated() - before < flat.numel()
