@@ -120,8 +120,8 @@ def _heads(name, H, Hk, D):
 
 def _scale(name, scale, D):
     s = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < s < math.inf:
-        raise ValueError(f"{name}: the scale has to be positive and finite, got {scale!r}")
+    if not 2.0 ** -126 <= s <= 2.0 ** 127:
+        raise ValueError(f"{name}: the scale has to be positive, 2^127 at most and a normal number in 32 bits, got {scale!r}")
     return s
 
 

@@ -311,7 +311,7 @@ static inline int window_attention_check(const char *name, int dtype, int b, int
     PA_REQUIRE(d > 0 && d <= 128 && d % 8 == 0, "%s: head width %d is not a multiple of 8 up to 128", name, d);
     PA_REQUIRE(left >= -1 && right >= -1 && left <= pa_attn::MAXLEN && right <= pa_attn::MAXLEN && sinks >= 0, "%s: bad window left=%d right=%d sinks=%d", name, left,
                right, sinks);
-    PA_REQUIRE(scale > 0.f && scale < INFINITY, "%s: the scale has to be positive and finite", name);
+    PA_REQUIRE(scale > 0.f && scale <= 0x1p127f, "%s: the scale has to be in (0, 2^127]", name);
     return PA_OK;
 }
 

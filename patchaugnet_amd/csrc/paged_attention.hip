@@ -318,7 +318,7 @@ PA_API int pa_paged_attention(int dtype, int b, int h, int hk, int d, const void
     if (rc != PA_OK) return rc;
     PA_REQUIRE(h > 0 && h % hk == 0, "pa_paged_attention: %d query heads do not share %d key heads evenly", h, hk);
     PA_REQUIRE(left >= -1 && left <= MAXLEN && sinks >= 0, "pa_paged_attention: bad window left=%d sinks=%d", left, sinks);
-    PA_REQUIRE(scale > 0.f && scale < INFINITY, "pa_paged_attention: the scale has to be positive and finite");
+    PA_REQUIRE(scale > 0.f && scale <= 0x1p127f, "pa_paged_attention: the scale has to be in (0, 2^127]");
     if (b == 0) return PA_OK;
     PA_REQUIRE(q && out && length && (width_ == 0 || table) && (pages == 0 || (k_pages && v_pages)), "pa_paged_attention: null tensor");
     PA_REQUIRE(alignment_of(dtype == PA_DT_F32 ? 4 : 2, {q, k_pages, v_pages, out, scratch}, {qb, qh, kp, kt, kh, vp, vt, vh}) == 16,

@@ -144,3 +144,18 @@ def test_first_tokens_behind_the_last_key_ask_for_no_splits(lib):
         for left in (-1, 0, 16, 300):
             assert g(1, n, m, 8, 8, 32, left, 0, 10 ** 6) == g(1, n, m, 8, 8, 32, left, 0, m), (n, m, left)
     assert g(1, 64, 64, 8, 8, 32, 16, 0, 10 ** 6) == 0
+
+
+def test_scales_that_leave_32_bits_are_refused(lib):
+    """The kernels multiply scores by scale log2(e) in 32 bits; in Python as a ValueError, whatever the number."""
+    buf = (ctypes.c_char * 4096)()
+    base = (ctypes.addressof(buf) + 15) // 16 * 16
+    p, at, z = ctypes.c_void_p(0), ctypes.c_void_p(base), (ctypes.c_void_p(base), 0, 32, 32)
+    for scale in (3e38, 2.4e38):
+        assert lib.pa_window_attention(0, 1, 1, 1, 1, 1, 32, *z, *z, *z, -1, 0, 0, scale, p, p, at, p, p, at, p) == -1
+        assert lib.pa_window_attention_backward(0, 1, 1, 1, 1, 1, 32, *z, *z, *z, at, p, at, *z, -1, 0, 0, scale, p, p, at, at, at, at, p) == -1
+        assert lib.pa_paged_attention(0, 1, 1, 1, 32, at, 0, 32, *z, *z, 1, 1, at, 1, at, -1, 0, scale, at, at, p) == -1
+    for scale in (3e38, 1e300, 1e-50, 0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError):
+            attention._scale("x", scale, 32)
+    assert attention._scale("x", None, 64) == 0.125 and attention._scale("x", 1e38, 64) == 1e38
