@@ -21,6 +21,7 @@ import math
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -358,6 +359,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, starts, *, counts=None):
     with _on(k.device):
         call("pa_paged_append", dt, B, T, Hk, D, ptr(k), *_strides(k), ptr(v), *_strides(v), ptr(k_pages), *_strides(k_pages), ptr(v_pages), *_strides(v_pages),
              k_pages.shape[0], k_pages.shape[1], ptr(table), table.shape[1], ptr(starts), ptr(counts))
+    increment_version((k_pages, v_pages))                      # a backward pass that saved rows of the pools refuses them
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, *, left=None, sinks=0, scale=None):

@@ -285,3 +285,17 @@ def test_refused_pools_are_not_copied():
             with pytest.raises(ValueError, match="16 bytes"):
                 call()
     assert torch.cuda.max_memory_allocated() - before < flat.numel()
+
+
+def test_gradients_do_not_read_stale_rows():
+    """window_attention over rows of a pool, then an append into it: the backward pass says so instead of using the new rows."""
+    from patchaugnet_amd.attention import paged_append, window_attention
+    q, k, v = _inputs(1, 32, 2, 2, 32, BF16)
+    kp, vp, table = _cache(k, v, 32, [32], spare=0)
+    leaf = q.unsqueeze(1).clone().requires_grad_()
+    out = window_attention(leaf, kp, vp, q_start=_i([31]))
+    paged_append(k[:, :1], v[:, :1], kp, vp, table, _i([5]))
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    with torch.inference_mode():
+        paged_append(k[:, :1], v[:, :1], kp.clone(), vp.clone(), table, _i([5]))
