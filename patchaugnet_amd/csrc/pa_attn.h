@@ -275,11 +275,15 @@ template <int KT> struct TileList {
     __device__ __forceinline__ int tile(int i) const { return i < nsk ? i : lo + i - nsk; }
 };
 
-// Waves of a workgroup, each with 32 rows (or keys).  Four share a tile's way into LDS; with two, the keys that a workgroup walks reach less beyond its
-// own rows and float32 needs fewer registers for tiles on their way.  Measured, us with four / two waves: forward bf16 4 x 4096 x 16 heads of 64, window
-// 512: 62 / 83; 16384 tokens of 128, window 1024: 748 / 832; float32 4 x 2048 x 8 of 64 and 128, window 256: 64 / 60 and 142 / 127; dk and dv of the
-// latter 209 / 184 and 454 / 447, of fp16 8 x 4096 x 8 of 96 with 64 keys either side 122 / 103, of bf16 4 x 2048 x 16 of 64, all keys: 193 / 236.
-static inline int waves_of(int es, long reach) { return es == 4 || reach < 256 ? 2 : 4; }
+// Waves of a workgroup, each with 32 rows (forward, dq) or 32 keys (dk and dv).  Four share a tile's way into LDS; with two, the keys (rows) that a workgroup
+// walks reach less beyond its own and float32 needs fewer registers for tiles on their way.  Measured, us with four / two waves:
+//   rows, bf16 forward, 8 x 4096 tokens, keys in reach 64 / 128 / 256 / 512: 8 heads of 64: 34, 34, 43, 63 / 31, 35, 45, 67; 16 of 128 over 4: 115, 125, 151, 209 /
+//   119, 132, 160, 226.  What two gain at a reach of 64 with as many key heads they lose elsewhere, so 16-bit rows take four.  float32 4 x 2048 x 8 of 64 and
+//   128, window 256: 64 / 60 and 142 / 127.
+//   keys, dk and dv: float32, the same two: 209 / 184 and 454 / 447; fp16 8 x 4096 x 8 of 96 with 64 keys either side 122 / 103; bf16 4 x 2048 x 16 of 64, all
+//   keys: 193 / 236.
+constexpr int row_waves(int es) { return es == 4 ? 2 : 4; }
+static inline int key_waves(int es, long reach) { return es == 4 || reach < 256 ? 2 : 4; }
 
 // 16-bit training passes over few (query, key) pairs multiply weights and dS as the sum of their rounding and the rest's.  Rounded once, dS adds as much to
 // the error of dq and dk as their own rounding does (1.41 times it together) where many pairs average out; up to 1.53 times it was seen below 2^22

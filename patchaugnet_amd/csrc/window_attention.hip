@@ -229,7 +229,7 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int es, int left, int right, 
 {
     const long G = H / Hk, rows = (long)N * G;
     Shape s;
-    s.waves = waves_of(es, UNBOUNDED);
+    s.waves = row_waves(es);
     s.nqt = pa_div_up(rows, 32 * s.waves);
     s.splits = 1;
     const long wgs = (long)B * Hk * s.nqt;
@@ -251,7 +251,7 @@ void launch_rows(const FwdArgs &a, hipStream_t st)
 template <typename T, int DT>
 int launch_fwd(const FwdArgs &a, hipStream_t st)
 {
-    constexpr int NW = sizeof(T) == 4 ? 2 : 4;
+    constexpr int NW = row_waves(sizeof(T));
     const bool fine = a.few || a.D <= 16;
     if (a.splits > 1) {
         if (fine) launch_rows<T, DT, NW, true, sizeof(T) == 2>(a, st);

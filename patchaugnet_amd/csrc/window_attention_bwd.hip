@@ -268,7 +268,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DT <= 64 ? 2 : 1) void d
     int e = 0;                                                 // lifted types: sums are 2^e dk and 2^P_LIFT dv
     if constexpr (lifted<T>()) {
         if (t0 < t1) {
-            const float *peak = a.peak + (size_t)w.bh * a.nqt * 4;       // of the four waves of the dq launch's workgroups
+            const float *peak = a.peak + (size_t)w.bh * a.nqt * row_waves(sizeof(T));       // one of every wave of the dq launch
             float most = 0.f;
             const int last = (min(ra + t1 * a.rt, rb) - 1) / 32;
             for (int x = (ra + t0 * a.rt) / 32 + l; x <= last; x += 64) most = fmaxf(most, peak[x]);
@@ -495,9 +495,9 @@ Shape shape_of(int B, int N, int M, int H, int Hk, int d, int es, int left, int 
 {
     Shape s;
     const long G = H / Hk, bh = (long)B * Hk, rows = (long)N * G;
-    s.qwaves = waves_of(es, UNBOUNDED);
+    s.qwaves = row_waves(es);
     s.nqt = pa_div_up(rows, 32 * s.qwaves);
-    s.kwaves = waves_of(es, (long)left + right);
+    s.kwaves = key_waves(es, (long)left + right);
     const int kb = 32 * s.kwaves, rt = width(d) * es >= 512 ? 32 : 64;
     s.rt = G <= rt ? rt / (int)G * (int)G : rt;
     s.nkt = pa_div_up(M, kb);
@@ -538,12 +538,12 @@ template <typename T, int DT>
 int launch_bwd(const BwdArgs &a, const Shape &s, hipStream_t st)
 {
     if constexpr (sizeof(T) == 4) {
-        if (a.nqt) launch_dq<T, DT, 2, false>(a, st);
+        if (a.nqt) launch_dq<T, DT, row_waves(4), false>(a, st);
         if (a.nkt) launch_dkv<T, DT, 2, false>(a, s.joined(), st);
     } else {
         if (a.nqt) {
-            if (a.few) launch_dq<T, DT, 4, true>(a, st);
-            else launch_dq<T, DT, 4, false>(a, st);
+            if (a.few) launch_dq<T, DT, row_waves(2), true>(a, st);
+            else launch_dq<T, DT, row_waves(2), false>(a, st);
         }
         if (a.nkt) {
             if (s.kwaves == 2 && a.few) launch_dkv<T, DT, 2, true>(a, s.joined(), st);
@@ -558,7 +558,7 @@ int launch_bwd(const BwdArgs &a, const Shape &s, hipStream_t st)
 }  // namespace
 
 // floats of scratch: delta (B H N), the largest |dS| of every 32 rows, then the partial sums of sliced walks
-static long front_floats(int b, int n, int h, int hk) { return pa_div_up((long)b * h * n, 4) * 4l + (long)b * hk * pa_div_up((long)n * (h / hk), 128) * 4; }
+static long front_floats(int b, int n, int h, int hk) { return pa_div_up((long)b * h * n, 4) * 4l + (long)b * hk * pa_div_up((long)n * (h / hk), 32 * row_waves(2)) * row_waves(2); }
 
 PA_API long pa_window_attention_backward_scratch_floats(int b, int n, int m, int h, int hk, int d, int left, int right, int sinks)
 {
