@@ -81,9 +81,9 @@ def _fits(t, align=16, far=1 << 62):
 
 def _rows(t, align=16, far=1 << 62):
     """t itself if it fits, else a contiguous copy."""
-    if _fits(t, align, far):
-        return t
-    return t.clone() if t.is_contiguous() else t.contiguous()
+    if t.is_contiguous():
+        return t if t.data_ptr() % align == 0 else t.clone()
+    return t if _fits(t, align, far) else t.contiguous()
 
 
 def _near(t, s):
@@ -96,11 +96,12 @@ def _unit(t):
 
 
 def _strides(t):
-    """Strides of all dimensions but the last.  A dimension with one entry may report any stride, in contiguous tensors too; the library would hold that
-    against its limits, so it gets the stride of the shape, or 0."""
+    """Strides of the first three of four dimensions (of fewer where t is not contiguous).  A dimension with one entry may report any stride, in contiguous
+    tensors too; the library would hold that against its limits, so it gets the stride of the shape, or 0."""
     if t.is_contiguous():
-        n = t.shape
-        return (n[1] * n[2] * n[3], n[2] * n[3], n[3]) if len(n) == 4 else (n[1] * n[2], n[2])
+        _, n, h, d = t.shape
+        row = h * d
+        return n * row, row, d
     return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
 
 
@@ -386,6 +387,6 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, left=None, sink
     out = q.new_empty(q.shape)
     with _on(q.device):
         scratch = _floats(_size("pa_paged_attention_scratch_floats", B, H, Hk, D, page, table.shape[1], left, sinks), q.device)
-        call("pa_paged_attention", dt, B, H, Hk, D, ptr(q), *_strides(q), ptr(k_pages), *_strides(k_pages), ptr(v_pages), *_strides(v_pages), P, page, ptr(table),
+        call("pa_paged_attention", dt, B, H, Hk, D, ptr(q), *((H * D, D) if q.is_contiguous() else _strides(q)), ptr(k_pages), *_strides(k_pages), ptr(v_pages), *_strides(v_pages), P, page, ptr(table),
              table.shape[1], ptr(lengths), left, sinks, scale, ptr(out), ptr(scratch))
     return out

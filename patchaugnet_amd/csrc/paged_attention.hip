@@ -272,23 +272,23 @@ int launch_paged(const PagedArgs &a, hipStream_t st)
     return 0;
 }
 
-// A thread copies 16 bytes of a new row of K and of V; more than 2^31 of them are dealt out in turns.
-__global__ __launch_bounds__(256) void append_kernel(long total, int tokens, int hk, int chunks, int es, const char *__restrict__ k, const char *__restrict__ v, long kb,
+// A thread copies 16 bytes of a new row of K and of V, pieces first .. total of all.
+__global__ __launch_bounds__(256) void append_kernel(long first, long total, int tokens, int hk, int chunks, int es, const char *__restrict__ k, const char *__restrict__ v, long kb,
                                                      long kn, long kh, long vb, long vn, long vh, char *__restrict__ kpages, char *__restrict__ vpages, long kp,
                                                      long kt, long kph, long vp, long vt, long vph, const int *__restrict__ table, long tb, int pages, int page,
                                                      int cap, const int *__restrict__ starts, const int *__restrict__ counts)
 {
-    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long)gridDim.x * 256) {
-        const int c = (int)(id % chunks);
-        const long rest = id / chunks;
-        const int g = (int)(rest % hk), t = (int)(rest / hk % tokens), b = (int)(rest / hk / tokens);
-        const long j = (long)starts[b] + t;
-        if ((counts && t >= counts[b]) || j < 0 || j >= cap) continue;
-        const int e = (int)j / page, at = (int)j - e * page, p = table[b * tb + e];
-        if ((u32)p >= (u32)pages) continue;
-        *reinterpret_cast<pa_u4 *>(kpages + (p * kp + at * kt + g * kph) * es + c * 16) = *reinterpret_cast<const pa_u4 *>(k + (b * kb + t * kn + g * kh) * es + c * 16);
-        *reinterpret_cast<pa_u4 *>(vpages + (p * vp + at * vt + g * vph) * es + c * 16) = *reinterpret_cast<const pa_u4 *>(v + (b * vb + t * vn + g * vh) * es + c * 16);
-    }
+    const long id = first + (long)blockIdx.x * 256 + threadIdx.x;
+    if (id >= total) return;
+    const int c = (int)(id % chunks);
+    const long rest = id / chunks;
+    const int g = (int)(rest % hk), t = (int)(rest / hk % tokens), b = (int)(rest / hk / tokens);
+    const long j = (long)starts[b] + t;
+    if ((counts && t >= counts[b]) || j < 0 || j >= cap) return;
+    const int e = (int)j / page, at = (int)j - e * page, p = table[b * tb + e];
+    if ((u32)p >= (u32)pages) return;
+    *reinterpret_cast<pa_u4 *>(kpages + (p * kp + at * kt + g * kph) * es + c * 16) = *reinterpret_cast<const pa_u4 *>(k + (b * kb + t * kn + g * kh) * es + c * 16);
+    *reinterpret_cast<pa_u4 *>(vpages + (p * vp + at * vt + g * vph) * es + c * 16) = *reinterpret_cast<const pa_u4 *>(v + (b * vb + t * vn + g * vh) * es + c * 16);
 }
 
 int paged_check(const char *name, int dtype, int b, int hk, int d, int pages, int page, int width)
@@ -358,10 +358,13 @@ PA_API int pa_paged_append(int dtype, int b, int tokens, int hk, int d, const vo
     PA_REQUIRE(alignment_of(es, {k, v, k_pages, v_pages}, {kb, kn, kh, vb, vn, vh, kp, kt, kph, vp, vt, vph}) == 16,
                "pa_paged_append: addresses and strides have to be multiples of 16 bytes");
     const long total = (long)b * tokens * hk * chunks;
-    const long groups = (total + 255) / 256, most = 1l << 23;
-    hipLaunchKernelGGL(append_kernel, dim3((unsigned)(groups < most ? groups : most)), dim3(256), 0, (hipStream_t)stream, total, tokens, hk, chunks, es, (const char *)k,
-                       (const char *)v, kb, kn, kh, vb, vn, vh, (char *)k_pages, (char *)v_pages, kp, kt, kph, vp, vt, vph, table, (long)width_, pages, page,
-                       width_ * page, starts, counts);
+    constexpr long most = 1l << 31;                            // pieces of a launch
+    for (long first = 0; first < total; first += most) {
+        const long n = total - first < most ? total - first : most;
+        hipLaunchKernelGGL(append_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, first, total, tokens, hk, chunks, es, (const char *)k,
+                           (const char *)v, kb, kn, kh, vb, vn, vh, (char *)k_pages, (char *)v_pages, kp, kt, kph, vp, vt, vph, table, (long)width_, pages, page,
+                           width_ * page, starts, counts);
+    }
     PA_CHECK_LAUNCH("pa_paged_append");
     return PA_OK;
 }
