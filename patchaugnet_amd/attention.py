@@ -2,17 +2,18 @@
 stay in view, and its form for one new token over a paged cache.
 
 Next to the grouped self-attention over a whole cloud (``backbone.SALayer``, ``train_ops.sa_attention_train``), whose cost grows with the square of the
-points: here a point in the serial order of its cloud (the order of ``pa_cloud_cellsort``, a space-filling curve, ...), or a submap in the stream
-of a drive, sees its neighbours within a window and the first ``sinks`` tokens.
+points: here a point in a serial order of its cloud (a space-filling curve, cells of a grid, ...; the caller brings it), or a submap in the stream of a drive,
+sees its neighbours within a window and the first ``sinks`` tokens.
 
   qk_norm_rotary      norm of every head of q and k, then the rotation by positions or coordinates          with gradients
   window_attention    prompts, clouds, training                                                                  with gradients
   paged_append        new keys and values into a paged cache
   paged_attention     one new token of every sequence over that cache
 
-Types: float32, float16, bfloat16 (sums, soft-max and norms in 32 bits).  Heads: ``H`` query heads share ``Hk`` key heads, ``H % Hk == 0``; query head
-``i`` reads key head ``i // (H // Hk)``.  Everything runs on the current stream of the tensors' device through libpatchaugnet_hip.so; there is no
-CPU form.
+Types: float32, float16, bfloat16.  Scores, maxima, sums and norms are held in 32 bits; the weights of the soft-max are rounded to the tensors' type for
+their products (16-bit results are off by up to 1.5 times their own rounding).  How work is split, and with it the last bits, goes by the sizes of the
+whole batch.  Heads: ``H`` query heads share ``Hk`` key heads, ``H % Hk == 0``; query head ``i`` reads key head ``i // (H // Hk)``.  Everything runs on the
+current stream of the tensors' device through libpatchaugnet_hip.so; there is no CPU form.
 """
 import contextlib
 import functools
@@ -207,7 +208,8 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, *, positions=None, inv_fr
       the first 2 A F elements of n turned in pairs by the angles positions[..., a] * inv_freq[a, f]
 
     inv_freq: float32 (F,) or (A, F): F frequencies for each of A axes; pair number a F + f.  positions: (N,) or (B, N) for one axis, (N, A) or
-    (B, N, A) for several, int32, int64 or float32 -- token numbers or coordinates.  Angles are reduced in 64 bits: far positions keep full accuracy.
+    (B, N, A) for several, int32, int64 or float32 -- token numbers or coordinates.  Angles are reduced in 64 bits: up to 2^27 radians they keep full 32-bit accuracy, beyond
+    that they are off by 2^-52 of their size.
     Pairs are elements (i, i + A F), with interleaved=True (2 i, 2 i + 1).  positions=None: the norm alone.  D up to 512, any strides.
     Gradients for q, k and the weights; positions and frequencies get none (a tensor of theirs that asks for one is refused)."""
     name = "qk_norm_rotary"
@@ -301,8 +303,8 @@ def window_attention(q, k, v, *, left=None, right=0, sinks=0, scale=None, length
                 q, k, v holds has no influence, NaN included.  Within a sequence a NaN or an infinity reaches rows that do not see it.
       q_start   int32 (B,): position of the first query (None: 0) -- the next part of a prompt, whose earlier keys lie in front of it in k and v.
     Values outside 0..M are clamped.  scale None: 1 / sqrt(D).  Strides are free except that a row is contiguous and starts at a multiple of 16 bytes
-    (other tensors are copied; so are those with 2^22 elements and more between two tokens or heads; H D up to 2^22).  Gradients for q, k, v, the same bits on every run; in the
-    16-bit types what the rounding of out left, a tensor of its size, is kept for them.  Weights and the gradients of scores are rounded to the tensors' type
+    (other tensors are copied; so are those with 2^22 elements and more between two tokens or heads; H D up to 2^22).  Gradients for q, k, v, all three
+    whichever are asked for, the same bits on every run; in the 16-bit types what the rounding of out left, a tensor of its size, is kept for them.  Weights and the gradients of scores are rounded to the tensors' type
     for the products; float16: brought into its range by powers of two first, so neither small gradients nor those that pass 65504 there are lost."""
     name = "window_attention"
     _check(name, q, k, v)

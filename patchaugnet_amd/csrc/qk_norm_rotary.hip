@@ -8,13 +8,14 @@
 //
 // Bound: bytes -- x and y (backward: x, dy and dx) once.  A few lanes hold a row: a lane has the two V-element pieces of its pairs (one row of 128
 // 16-bit elements: 8 lanes with 2 x 16 bytes each), so the mean square is the only exchange between lanes.  The rotation's sines and cosines are the
-// expensive part (64-bit range reduction: positions of 10^6 keep full accuracy); a workgroup computes those of its tokens once, into LDS, for all
+// expensive part (64-bit range reduction: angles up to 2^27 keep full accuracy); a workgroup computes those of its tokens once, into LDS, for all
 // query and key heads.  Everything between load and store is 32-bit, rounded once.
 //
 // Measured, forward / backward / weights: bf16 8 x 4096 tokens, 16 + 4 heads of 128: 75 / 129 / 5 us (336 and 503 MB: 4.5 and 3.9 TB/s; a copy: 4.9);
 // float32 18 x 1024, 8 + 8 heads of 64, three axes: 28 / 47 / 4 us.  Addresses and angles once per token (64-bit products per row cost 224 us backward),
 // the next row in flight.  A piece is 16 bytes wide; where the number of pairs is no multiple of that, lanes keep pieces of consecutive elements and the
-// pairs are exchanged through LDS (2.0 to 3.5 TB/s); where the rows themselves do not start at 16 bytes, pieces are narrower (heads of 66: 0.7 TB/s).
+// pairs are exchanged through LDS (1.5 to 3.5 TB/s); where the rows themselves do not start at 16 bytes, pieces are narrower (16-bit heads of 66, 33 pairs: 2 bytes,
+// 0.7 TB/s).
 //
 // The weight gradients are sums over all tokens and heads: per lane in registers over a workgroup's tokens, then across the workgroup, then by a
 // second launch over the workgroups' rows, always in the same order.
@@ -66,7 +67,7 @@ __device__ __forceinline__ float2 turn(double x)
 {
     const double q = x * 0.63661977236758134308;                // quarter turns
     const double n = __builtin_rint(q);
-    // x / (pi / 2) is rounded at 2^-53 of its size; the frequencies are 32-bit numbers, so x itself is exact
+    // x and x / (pi / 2) are each rounded at 2^-53 of their size: the angle is off by 2^-52 |x|, less than 32 bits resolve up to |x| = 2^27
     const float f = (float)(q - n);
     float s, c;
     sincospif(0.5f * f, &s, &c);

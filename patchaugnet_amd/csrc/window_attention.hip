@@ -10,19 +10,21 @@
 //
 // Roundings: s, maximum, sum and o are 32-bit; P is rounded to the type of V for the second product (16-bit types), with P <= 2^8 by the running
 // maximum, which is only moved when a row's maximum grows by more than 2^8 (the quotient is the same for any reference value).  Where a backward pass
-// follows, its delta is a difference that magnifies the error of o: what the rounding of o leaves is handed on beside it, and for heads of 8 and 16 (where
-// dq was off by 1.50 to 1.52 times the rounding of the result, now 1.47; wider ones by 1.48 at most) and few pairs (few_pairs()) P is multiplied as the
-// sum of its rounding and the rest's -- without gradients too, so that out has the same bits with and without.  4 x 4096 tokens, 16 heads over 4 in a tile
-// 32 wide, window 512: 45 us, in two parts 60.
+// follows, its delta is a difference that magnifies the error of o: what the rounding of o leaves is handed on beside it, and for heads of 8 and 16 (their
+// dq is off by up to 1.58 times the rounding of the result, wider heads' by 1.5) and few pairs (few_pairs()) P is multiplied as the sum of its rounding and
+// the rest's -- without gradients too, so that out has the same bits with and without.  4 x 4096 tokens, 16 heads over 4 in a tile 32 wide, window 512:
+// 45 us, in two parts 60.
 //
-// Measured: bf16 4 x 16384 tokens, 16 heads of 128 over 4, window 1024: 688 us = 780 TFLOP/s of visible pairs (a library product of that type: 1219;
+// Measured: bf16 4 x 16384 tokens, 16 heads of 128 over 4, window 1024: 665 us = 805 TFLOP/s of visible pairs (a library product of that type: 1219;
 // 12 % of the work is keys of tiles that a row does not see); 4 x 4096, 16 heads of 64 over 4, window 512: 60 us = 540 (68 with what the rounding of out
-// leaves, for a backward pass); all keys of 4 x 2048, 16 heads of 64: 91 us = 755.  A 32 x 32 part costs 512 cycles of MFMA (width 128), about 600 of
-// vector instructions (256 of them the 16 exponentials) and 512 of the CU's LDS reads, on pipes that overlap only between the two to four waves of a
-// SIMD: that is the bound.  Reading ahead by one product within a wave (scores of the next part beside the exponentials of this one) cost more in
-// registers than it hid (80 against 65 us at width 64).
+// leaves, for a backward pass); all keys of 4 x 2048, 16 heads of 64: 91 us = 755.
+// Bound, by counters: matrix and vector work of the two waves of a SIMD mostly follow one another.  Width 128, window 1024: matrix units busy 39 % of the
+// time, vector units 46 %, LDS 20 % and free of bank conflicts, 1.9 waves per SIMD; 133 vector and 59 scalar instructions for a 32 x 32 part of 16 MFMA.
+// Width 64, window 512: vector 50 %, matrix 21 %, LDS 10 %; 136 vector and 66 scalar instructions for a part of 8 MFMA.  Reading ahead by one product
+// within a wave (scores of the next part beside the exponentials of this one) cost more in registers than it hid (80 against 65 us at width 64).
 // float32 72 x 1024, 8 heads of 64, all keys: 1245 us = 124 of the 153 TFLOP/s of a library product; 18 x 1024, 8 heads of 32, 128 keys either side: 76 us =
-// 60: a quarter of the keys in its parts are out of view, and it is nine waves per SIMD in all, whose start and end nothing covers.
+// 60: a quarter of the keys in its parts are out of view, and it is 4.5 waves per SIMD in all, whose start and end nothing covers (matrix units busy 45 %,
+// vector 17 %, LDS 4 %).
 #include "pa_attn.h"
 
 using namespace pa_attn;

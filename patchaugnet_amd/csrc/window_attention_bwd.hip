@@ -14,12 +14,15 @@
 //
 // Roundings: P and dS are rounded to the operand type for the second products (16-bit types; the sum of two parts for few pairs, few_pairs()); the scale
 // is applied to the 32-bit sums, so that dS is rounded before it gets smaller.  delta takes o as the forward pass had it before it was rounded
-// (out + low): dP - delta is small beside delta, and with the rounded o alone dq and dk were off by 1.6 times the rounding of the result, now 1.42 to 1.47.
+// (out + low): dP - delta is small beside delta, and with the rounded o alone dq and dk were off by 1.6 times the rounding of the result, now 1.4 to 1.5 (heads of 8: up to 1.58).
+// float16 has its P and dS lifted into its range besides (lifted()), which costs 5 to 8 % of such a pass; without it gradients of 1e-3 had dq and dk off by 1.5 to 11.
 //
 // Measured, dq / dk and dv / join: bf16 4 x 4096 tokens, 16 heads of 64 over 4, window 512: 81 / 113 / 5 us (600 / 575 TFLOP/s of visible pairs); all keys of
-// 4 x 2048, 16 heads of 64: 114 / 157 us (900 / 870; a library product: 1219); 2 x 8192, 16 of 128 over 4, window 1024: 215 / 466 / 7 us; float32
-// 18 x 1024, 8 heads of 32, 128 keys either side: 109 / 155 / 9 us.  Bound by MFMA and LDS reads together (16 KB read for 16 to 32 products of a wave).
-// dk, dv at width 128 holds 390 registers, one wave per SIMD: there nothing hides a wave's exponentials, and its rate is 550.
+// 4 x 2048, 16 heads of 64: 114 / 157 us (900 / 870; a library product: 1219); 2 x 8192, 16 of 128 over 4, window 1024: 226 / 437 / 7 us; float32
+// 18 x 1024, 8 heads of 32, 128 keys either side: 110 / 158 / 9 us; fp16 4 x 4096 tokens, 16 heads of 64 over 4, window 512: 89 / 124 / 5.
+// Bound, by counters.  dq as the forward pass: at width 64 and window 512 vector units busy 46 %, matrix units 28 %, LDS 14 %, 2.2 waves per SIMD.  dk, dv there:
+// 1.6 waves per SIMD, which wait 45 % of their time; vector 32 %, matrix 25 %, LDS 20 %.  At width 128 it holds 390 registers, one wave per SIMD: nothing hides a
+// wave's exponentials and reads (matrix 24 %, vector 20 %, LDS 15 %, 47 % waiting), and its rate is 580.  float32: matrix 44 to 47 %, vector 12, LDS 4 to 6.
 #include "pa_attn.h"
 
 using namespace pa_attn;
