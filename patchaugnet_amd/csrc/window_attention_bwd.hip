@@ -150,7 +150,7 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
 #pragma unroll
                 for (int r = 1; r < 16; ++r) mx = larger(mx, fabsf(s[r]));
                 mx = larger(mx, other_half(mx));
-                most = fmaxf(most, mx);
+                most = fmaxf(most, mx);                        // NaN is passed over
                 if (__any(mx > top)) {                         // the first dS that is not 0, or one that passes 2^15
                     const int up = mx > top ? min(e + 10 - exponent(mx), MAX_LIFT) : e;
                     const float by = pow2(up - e);
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DT>())) void dq_kernel(
         if (it + 1 < tiles.n) step(it + 1, k1, v1, k0, v0);
     }
     if constexpr (lifted<T>()) {
-        most *= pow2(-e);
+        most = most < INFINITY ? most * pow2(-e) : 0.f;        // a row that is lost already does not decide for the others
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
         if (l == 0) a.peak[((size_t)bh * a.nqt + qt) * NW + wave] = most;

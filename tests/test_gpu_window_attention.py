@@ -410,3 +410,22 @@ def test_more_joined_keys_than_a_launch_holds():
         for n in ("dk", "dv"):
             assert val[n][:, part].any()
             assert _ratios({n: got[n]}, {n: val[n]}, part)[n] <= 2.0, (n, part)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("what", ["inf", "nan"])
+def test_a_broken_gradient_stays_with_its_keys(dtype, what):
+    """An infinity or NaN in one row's incoming gradient: keys in later 32-key parts, which do not see the row, keep their dk and dv, other rows their dq."""
+    q, k, v, do = _qkv(1, 1500, 1500, 2, 1, 64, dtype, seed=15)
+    do = do * 64
+    do[0, 63] = 0
+    do[0, 90:] *= 2.0 ** -10                                    # the largest dS that keys from 64 on meet stand beside the broken row, or just behind
+    v[0, :32, 0, 7], v[0, 32:64, 0, 7] = 9, -0.5                # the gradients of the row's weights: NaN in its first part, minus infinity in its second
+    val, _ = reference(q, k, v, None, 0, 0, None, None, None, do)
+    do[0, 63, 1, 7] = float(what)
+    got = _run(q, k, v, do, None, 0, 0)
+    late = slice(64, None)
+    for n in ("dq", "dk", "dv"):
+        assert torch.isfinite(got[n][:, late]).all(), n
+        assert (got[n][:, late].double() - val[n][:, late]).norm() <= 4 * (torch.finfo(dtype).eps / 2 if dtype != F32 else 1e-6) * val[n][:, late].norm(), n
+    assert not torch.isfinite(got["dq"][0, 63, 1]).all()
